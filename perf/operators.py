@@ -320,10 +320,11 @@ def _rows_of_pages(pages):
     def nibbles(b):
         return torch.stack([level[(b & 15).long()], level[(b >> 4).long()]], -1)
 
-    # K: 16-key blocks, halves of the row, quarters of a group, keys, groups of the half, 8 dims
-    k = nibbles(pages[..., :cut].reshape(n, nkv, 4, 2, 4, 16, 4, 4)).reshape(n, nkv, 4, 2, 4, 16, 4, 8)
-    k = k.permute(0, 2, 5, 1, 3, 6, 4, 7).reshape(n * PAGE, nkv, 8, 32)
-    ks = pages[..., cut:half].reshape(n, nkv, PAGE, 8).permute(0, 2, 1, 3).reshape(n * PAGE, nkv, 8)
+    # K: 16-key blocks, halves of the row, groups of the half, keys, the group's dims
+    k = nibbles(pages[..., :cut].reshape(n, nkv, 4, 2, 4, 16, 16)).reshape(n, nkv, 4, 2, 4, 16, 32)
+    k = k.permute(0, 2, 5, 1, 3, 4, 6).reshape(n * PAGE, nkv, 8, 32)
+    # its scales: 32-key blocks, groups of the half, keys, 16-key block, half of the row
+    ks = pages[..., cut:half].reshape(n, nkv, 2, 4, 16, 2, 2).permute(0, 2, 5, 4, 1, 6, 3).reshape(n * PAGE, nkv, 8)
     # V: 32-key blocks, pairs of groups, quarters, pairs of dims, group of the pair, 16-key block, key of the quarter
     v = nibbles(pages[..., half:half + cut].reshape(n, nkv, 2, 4, 4, 16, 2, 2, 4))
     v = v.permute(0, 2, 7, 4, 8, 1, 3, 6, 5, 9).reshape(n * PAGE, nkv, 8, 32)
@@ -498,11 +499,11 @@ def _page_offsets():
     """Byte offset and shift of the code, and byte offset of the scale, of each (token of a page, dim) of K and of V."""
     t, d = np.meshgrid(np.arange(PAGE), np.arange(HD), indexing="ij")
     grp, r = d // 32, d % 32
-    kb = (((t // 16 * 2 + grp // 4) * 4 + r // 8) * 16 + t % 16) * 16 + grp % 4 * 4 + r % 8 // 2
+    kb = (((t // 16 * 2 + grp // 4) * 4 + grp % 4) * 16 + t % 16) * 16 + r // 2
     lane = t % 16 // 4 * 16 + r // 2
     vb = ((t // 32 * 4 + grp // 2) * 64 + lane) * 16 + grp % 2 * 8 + t % 32 // 16 * 4 + t % 4
     cut, half = PAGE * HD // 2, HEAD_BYTES // 2
-    ks = cut + t * 8 + grp
+    ks = cut + ((t // 32 * 4 + grp % 4) * 16 + t % 16) * 4 + t % 32 // 16 * 2 + grp // 4
     vs = half + cut + ((t // 32 * 4 + t % 16 // 4) * 8 + grp) * 8 + t % 32 // 16 * 4 + t % 4
     return [torch.from_numpy(x).to(DEV) for x in (kb, 4 * (d % 2), ks, half + vb, 4 * (d % 2), vs)]
 
