@@ -39,6 +39,8 @@ SYMBOLS = (
     "fn_gdn_verify_dev", "fn_advance_by_dev", "fn_gdn_block_xab_dev",
     "fn_attn_noalloc_dev", "fn_dev_status", "fn_model_dims", "fn_gemv_group_dev", "fn_stage_events",
     "fn_bench_gdn", "fn_bench_attn",
+    "fn_page_plan_dev", "fn_page_release_dev", "fn_kv4_page_bytes", "fn_kv4_pack_dev", "fn_kv4_unpack_dev",
+    "fn_attn_kv4_dev", "fn_attn_kv4_work_bytes", "fn_attn_kv4_nsplit",
 )
 
 # the shapes fn_model_dims writes, in order (include/faie2fn.h section 6)
@@ -46,7 +48,7 @@ MODEL_DIMS = ("D", "NL", "NH", "NKV", "HD", "NROT", "NE", "NEU", "FFE", "FFS", "
               "attn_every", "HC", "HCR", "IXH", "IXD", "top", "VOCAB", "PLE_LAYERS", "PLE_HEADS", "PLE_HD")
 
 # status bits of fn_dev_status (include/faie2fn.h)
-STATUS_POS, STATUS_KR = 1, 2
+STATUS_POS, STATUS_KR, STATUS_PAGE, STATUS_ROWS, STATUS_VALUE = 1, 2, 4, 8, 16
 
 # bytes of the device array fn_attn_noalloc_dev takes its workspace from (FN_NOALLOC_SCRATCH_BYTES)
 NOALLOC_SCRATCH_BYTES = 32 << 20
@@ -155,6 +157,15 @@ class FN:
         d.fn_gemv_work_bytes.argtypes = [u32, i, i, i]
         d.fn_gemv_dev.argtypes = [u32, VP, i, i, VP, i, VP, VP, sz, VP]
         d.fn_gemv_group_dev.argtypes = [i, VP, VP, i, VP, VP, i, VP, VP]
+        d.fn_page_plan_dev.argtypes = [i] * 4 + [VP] * 10
+        d.fn_page_release_dev.argtypes = [i] * 3 + [VP] * 6
+        d.fn_kv4_page_bytes.restype = sz
+        d.fn_kv4_page_bytes.argtypes = [i, i]
+        d.fn_kv4_pack_dev.argtypes = d.fn_kv4_unpack_dev.argtypes = [i] * 4 + [VP] * 5
+        d.fn_attn_kv4_dev.argtypes = [i] * 6 + [f, f, i, i] + [VP] * 11 + [i, VP, sz, VP, VP]
+        d.fn_attn_kv4_work_bytes.restype = sz
+        d.fn_attn_kv4_work_bytes.argtypes = [i] * 6
+        d.fn_attn_kv4_nsplit.argtypes = [i] * 5
 
     def check(self, rc):
         if rc != 0:
@@ -416,6 +427,40 @@ class FN:
         pk = (VP * n)(*packed)
         yp = (VP * n)(*ys)
         self.check(self.d.fn_gemv_group_dev(n, ty, rw, cols, pk, x, nt, yp, stream))
+
+    # ---- a packed batch of requests (include/faie2fn.h section 3c; device addresses as above) ----
+    def page_plan_dev(self, B, T, max_blocks, npages, past, nnew, free_list, free_top, free_left, table, cu, slot, seq,
+                      stream=0):
+        """Page table entries, cu [B+1], slot [T] and seq [T] for nnew[b] new tokens a request."""
+        self.check(self.d.fn_page_plan_dev(B, T, max_blocks, npages, past, nnew, free_list, free_top, free_left, table,
+                                           cu, slot, seq, stream))
+
+    def page_release_dev(self, B, max_blocks, npages, done, past, free_list, free_top, table, stream=0):
+        """The pages of the requests with done[b] != 0 back on the stack."""
+        self.check(self.d.fn_page_release_dev(B, max_blocks, npages, done, past, free_list, free_top, table, stream))
+
+    def kv4_page_bytes(self, nkv, hd=256):
+        return int(self.d.fn_kv4_page_bytes(nkv, hd))
+
+    def kv4_pack_dev(self, n, nkv, npages, slot, k, v, cache, stream=0, hd=256):
+        """Rows k, v [n][nkv][hd] into the slots of the 4-bit cache."""
+        self.check(self.d.fn_kv4_pack_dev(n, nkv, hd, npages, slot, k, v, cache, stream))
+
+    def kv4_unpack_dev(self, n, nkv, npages, slot, cache, k, v, stream=0, hd=256):
+        """The values that the slots of the 4-bit cache stand for, as rows k, v [n][nkv][hd]."""
+        self.check(self.d.fn_kv4_unpack_dev(n, nkv, hd, npages, slot, cache, k, v, stream))
+
+    def attn_kv4_work_bytes(self, B, T, nq, nkv, nsplit, hd=256):
+        return int(self.d.fn_attn_kv4_work_bytes(B, T, nq, nkv, hd, nsplit))
+
+    def attn_kv4_nsplit(self, B, T, nq, nkv, ctx):
+        return int(self.d.fn_attn_kv4_nsplit(B, T, nq, nkv, ctx))
+
+    def attn_kv4_dev(self, B, T, nq, nkv, max_blocks, npages, past, cu, table, slot, seq, qg, k, v, wq, wk, cache,
+                     nsplit, work, work_bytes, og, stream=0, hd=256, nrot=64, theta=1e7, eps=1e-6):
+        """The attention layer of a packed batch over the 4-bit paged cache."""
+        self.check(self.d.fn_attn_kv4_dev(B, T, nq, nkv, hd, nrot, float(theta), float(eps), max_blocks, npages, past, cu,
+                                          table, slot, seq, qg, k, v, wq, wk, cache, nsplit, work, work_bytes, og, stream))
 
     # ---- path engine ----
     def path_init(self, B, nl, attn_every=4, nkh=16, nvh=32, nq=16, nkv=2, max_ctx=4096, head_map=0, gate_act=0,

@@ -209,6 +209,9 @@ int fn_attn_noalloc_dev(int B, int nq, int nkv, int hd, int nrot, float theta, f
  * themselves and fail with an fn_error() message. */
 #define FN_STATUS_POS 1u  /* attention: a new token's position pos[b] + t outside [0, max_ctx) */
 #define FN_STATUS_KR 2u   /* verify: kr[b] outside [0, rnt] */
+#define FN_STATUS_PAGE 4u   /* paged cache: the free pages ran out, or a page or slot number outside the cache */
+#define FN_STATUS_ROWS 8u   /* packed batch: a negative count, rows beyond T, or cu / seq that do not fit together */
+#define FN_STATUS_VALUE 16u /* 4-bit cache: an infinity or NaN in a row to be held (its group of 32 is stored as zeros) */
 int fn_dev_status(int clear);
 
 /* pos[b] += nt for b < B, on the stream (the reference's k_advance, faie2fn.cu:1905). */
@@ -273,6 +276,59 @@ int fn_test_attn_qsa(int B, int nq, int nkv, int hd, int nrot, float theta, floa
                      const int32_t *pos, const float *qg, const float *k, const float *v, const float *wq,
                      const float *wk, float *Kc, float *Vc, const float *iqk, const float *wqn, const float *wkn,
                      float *IKc, int top, int nsplit, float *og, float *scores, uint8_t *mask);
+
+/* ======================================================================================================
+ * 3c. Serving a packed batch (new; no counterpart in the reference, which decodes one sequence): requests of different
+ *     lengths in one call.  Request b's new tokens are rows cu[b] .. cu[b + 1] - 1 of every per-token array of T rows; rows
+ *     from cu[B] on are left as they were.  past [B] are the tokens that each request already has (0 for a new one).
+ *     Nothing is allocated and no memset is recorded; a call can be captured into a graph and replayed with new
+ *     contents of its buffers.  What the device finds wrong is recorded in the status word (fn_dev_status).
+ * ====================================================================================================== */
+
+/* Page tables.  The cache is npages pages of 64 tokens; table [B][max_blocks] names the page of each 64-token block of
+ * a request (its first ceil(past / 64) entries stand on entry; other entries may hold anything).  For nnew [B] new
+ * tokens: pages for the blocks that become needed are taken from the end of the stack free_list [npages], whose count is
+ * free_top[0], in request order, block order, and entered in the table; free_left[0] is the count that is left
+ * (free_left may be free_top: the stack then moves on; apart, the call can be repeated).  Written: cu [B + 1]; for each
+ * of T rows slot [T] = page * 64 + row of the page and seq [T] = its request (-1 in rows from cu[B] on).  A block that
+ * gets no page (none is left, or it lies past max_blocks) has table entry -1 (none past max_blocks) and its tokens slot
+ * -1: not cached, and the status word says so.  New tokens beyond T rows are cut off.  B 1..8000. */
+int fn_page_plan_dev(int B, int T, int max_blocks, int npages, const int32_t *past, const int32_t *nnew,
+                     const int32_t *free_list, const int32_t *free_top, int32_t *free_left, int32_t *table, int32_t *cu,
+                     int32_t *slot, int32_t *seq, void *stream);
+
+/* The pages of every request with done[b] != 0 (the blocks of past[b] tokens) go back on the stack, in request order,
+ * block order; its table entries become -1 and past[b] 0.  Requests that end must not share pages. */
+int fn_page_release_dev(int B, int max_blocks, int npages, const int32_t *done, int32_t *past, int32_t *free_list,
+                        int32_t *free_top, int32_t *table, void *stream);
+
+/* 4-bit cache: keys and values as e2m1 codes with one power-of-two scale for 32 dims (4.25 bits a value), in pages of 64
+ * tokens; a page of one kv head is 17408 bytes (8192 of K codes, 512 of K scales, then V's), a page its heads one after
+ * the other.  The scale is the least power of two (2^-100 .. 2^125) that leaves the group's largest value off by at most
+ * half a step; codes are the nearest, ties to even.  fn_kv4_page_bytes: bytes of a page (0 if not built; hd 256). */
+size_t fn_kv4_page_bytes(int nkv, int hd);
+
+/* Rows k, v [n][nkv][hd] (keys already normalised and rotated) into slots slot [n], and back as the values that they stand
+ * for.  A slot of -1 is passed over (unpack leaves its row as it was).  k, v and cache 16-byte aligned; the slots of one
+ * pack are different. */
+int fn_kv4_pack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, const float *k, const float *v,
+                    uint8_t *cache, void *stream);
+int fn_kv4_unpack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, const uint8_t *cache, float *k, float *v,
+                      void *stream);
+
+/* The attention layer of fn_attn_dev on a packed batch and the 4-bit paged cache: qg [T][nq][2][hd], k, v [T][nkv][hd],
+ * og [T][nq][hd]; table, slot, seq and cu as fn_page_plan_dev leaves them.  Token t of request b at position
+ * past[b] + t - cu[b]: its normalised, rotated key and its value are written to slot[t] in 4 bits; its queries attend
+ * the request's keys up to its own position as the cache holds them (a block whose table entry is outside the cache is
+ * passed over; a query that finds no key gets zeros).  The rotation's angle is taken in 64 bits.  nq / nkv any whole number.
+ * nsplit: key splits of a row (fn_attn_kv4_nsplit: the choice for contexts of up to ctx keys).  All arrays but the
+ * int32 ones 16-byte aligned; work: fn_attn_kv4_work_bytes() bytes. */
+int fn_attn_kv4_dev(int B, int T, int nq, int nkv, int hd, int nrot, float theta, float eps, int max_blocks, int npages,
+                    const int32_t *past, const int32_t *cu, const int32_t *table, const int32_t *slot,
+                    const int32_t *seq, const float *qg, const float *k, const float *v, const float *wq,
+                    const float *wk, uint8_t *cache, int nsplit, void *work, size_t work_bytes, float *og, void *stream);
+size_t fn_attn_kv4_work_bytes(int B, int T, int nq, int nkv, int hd, int nsplit);
+int fn_attn_kv4_nsplit(int B, int T, int nq, int nkv, int ctx);
 
 /* ======================================================================================================
  * 4. Path engine (new): the reference's Engine + layer_forward + forward (faie2fn.cu:1937-2031, 2370-2490) for
