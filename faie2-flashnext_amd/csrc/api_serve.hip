@@ -50,3 +50,25 @@ FN_API int fn_attn_kv4_dev(int B, int T, int nq, int nkv, int hd, int nrot, floa
                   wq, wk, cache, work, work_bytes, og};
     return fn::kv4_attn_launch(p, (hipStream_t) stream);
 }
+
+FN_API size_t fn_gdn_chunk_work_bytes(int B, int T, int nkh, int nvh) {
+    if (B < 1 || T < 1 || nkh < 1 || nvh < 1) return 0;
+    return fn::gdn_chunk_work_bytes(B, T, nkh, nvh);
+}
+
+FN_API int fn_gdn_core_chunk_dev(int B, int T, int nkh, int nvh, int dk, int dv, int head_map, const int32_t *cu,
+                                 const float *q, const float *k, const float *v, const float *beta, const float *g,
+                                 float *S, float *o, void *work, size_t work_bytes, void *stream) {
+    fn::GdnChunk p{B, T, nkh, nvh, dk, dv, head_map, cu, q, k, v, beta, g, S, o, work, work_bytes};
+    return fn::gdn_chunk_launch(p, (hipStream_t) stream);
+}
+
+FN_API int fn_gdn_block_chunk_dev(int B, int T, int nkh, int nvh, int dk, int dv, int head_map, int gate_act, int ring,
+                                  const int32_t *cu, const int32_t *pos, const float *qkv, const float *conv_w,
+                                  float *conv_ring, const float *ab, const float *dt_bias, const float *ssm_a, float *S,
+                                  const float *z, const float *norm_w, float eps, float *out, void *work,
+                                  size_t work_bytes, void *stream) {
+    fn::GdnChunk p{B, T, nkh, nvh, dk, dv, head_map, cu, nullptr, nullptr, nullptr, nullptr, nullptr, S, out, work,
+                   work_bytes, true, gate_act, ring, eps, pos, qkv, conv_w, conv_ring, ab, dt_bias, ssm_a, z, norm_w};
+    return fn::gdn_chunk_launch(p, (hipStream_t) stream);
+}

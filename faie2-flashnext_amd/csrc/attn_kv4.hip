@@ -1,6 +1,7 @@
 // GQA attention of a packed ragged batch over the 4-bit paged cache: q/k RMSNorm + partial RoPE, append, online softmax,
 // sigmoid gate.  One call takes requests of one new token (decode), a few (verify) and whole prompts together.
 #include "kv4.cuh"
+#include "serve.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -43,26 +44,6 @@ struct Kv4Args {
     unsigned *status;
     double freq[MAXROT / 2];
 };
-
-// The rows of a request (tokens x query heads of a kv head) are cut in items of RT rows.  Item numbers: request b has
-// those from cu[b] grp / RT + b on, which leaves each request at least as many as it needs without a sum over the
-// requests; the spare ones are empty.
-__device__ __forceinline__ int first_item(const Kv4Args &a, int b, int rt) {
-    return (int) ((long long) a.cu[b] * a.grp / rt) + b;
-}
-// the last request whose items start at or before `item`: every lane looks at one of 64 of those left
-__device__ __forceinline__ int request_of(const Kv4Args &a, int item, int rt) {
-    int lo = 0, n = a.B;
-    const int lane = threadIdx.x & 63;
-    while (n > 1) {
-        const int step = (n + 63) / 64, i = lane * step;
-        const bool le = i < n && first_item(a, lo + i, rt) <= item;
-        const int k = max(1, __popcll(__ballot(le))) - 1;
-        lo += k * step;
-        n = min(step, n - k * step);
-    }
-    return __builtin_amdgcn_readfirstlane(lo);
-}
 
 // One token: sines and cosines of its position, its keys and values into their page, its queries as operands.
 template <int RT>
@@ -180,7 +161,7 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
         int e0 = (int) (u >> 23) - 127 - 2 + ((u & 0x7fffffu) > 0x700000u);
         e0 = max(e0, EMIN);
         const int g = h / a.grp, row = (t - a.cu[b]) * a.grp + (h - g * a.grp);
-        const int item = first_item(a, b, RT) + row / RT;
+        const int item = first_item(a.cu, b, a.grp, RT) + row / RT;
         uint8_t *dst = a.Q + (((size_t) g * a.items + item) * (RT / 16) + row % RT / 16) * QBLK;
         const int uh = gi >> 2, ln = (gi & 3) * 16 + row % 16;
         const bool st = on && item < a.items;
@@ -226,16 +207,6 @@ __device__ __forceinline__ v4f mma_v(const v4u &a, const v4u &b, v4f c) {
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), bf16x2));
 }
-// values of lane l ^ 16, l ^ 32 folded in
-__device__ __forceinline__ float max_quarters(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float sum_quarters(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
-}
-
 constexpr float SM_SCALE = 0.0625f * 1.4426950408889634f;  // 1 / sqrt(HD), and the softmax in powers of two
 constexpr float SLACK = 8.0f * 16.0f;                      // growth of a row's largest raw score that moves its reference
 constexpr float PUP = 16.0f;                               // probabilities times 2^16: the parts of the least ones stay normal
@@ -256,8 +227,8 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_kv4(const Kv4Args a) {
     __shared__ float wm[WAVES][RT], wl[WAVES][RT];
     const int sp = blockIdx.x, g = blockIdx.y, item = a.items - 1 - (int) blockIdx.z;  // the longest rows first
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int b = request_of(a, item, RT);
-    const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r0 = (item - first_item(a, b, RT)) * RT;
+    const int b = request_of(a.cu, a.B, item, a.grp, RT);
+    const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r0 = (item - first_item(a.cu, b, a.grp, RT)) * RT;
     const int rows = n * a.grp;
     if (c0 < 0 || r0 < 0 || r0 >= rows) return;
     const int past = a.past[b], cap = a.mb * PG;
@@ -505,8 +476,8 @@ template <int RT>
 __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
     const int item = blockIdx.x / (RT / 4), g = blockIdx.y, lane = threadIdx.x & 63;
     const int row = blockIdx.x % (RT / 4) * 4 + (threadIdx.x >> 6);
-    const int b = request_of(a, item, RT);
-    const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r = (item - first_item(a, b, RT)) * RT + row;
+    const int b = request_of(a.cu, a.B, item, a.grp, RT);
+    const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r = (item - first_item(a.cu, b, a.grp, RT)) * RT + row;
     if (c0 < 0 || r < 0 || r >= n * a.grp) return;
     const size_t at0 = ((size_t) item * a.nkv + g) * a.nsplit * RT + row;
     float M = -INFINITY;
@@ -531,7 +502,6 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
 
 // 16-row blocks an item: one where the requests have few rows (decode), two otherwise
 int row_blocks(int B, int T, int grp) { return (long long) T * grp <= 16ll * B ? 1 : 2; }
-size_t item_count(int B, int T, int grp, int rt) { return (size_t) ((long long) T * grp / rt) + B; }
 
 }  // namespace
 

@@ -1,0 +1,41 @@
+// Device helpers of the operators that serve a packed batch.
+#pragma once
+
+#include "serve.h"
+
+namespace fn {
+
+// The rows of a request (its tokens times `mul`) are cut in items of `div` rows.  Item numbers: request b has those from
+// cu[b] mul / div + b on, which leaves each request at least as many as it needs without a sum over the requests; the
+// spare ones are empty.
+__device__ __forceinline__ int first_item(const int32_t *cu, int b, int mul, int div) {
+    return (int) ((long long) cu[b] * mul / div) + b;
+}
+// the last request whose items start at or before `item`: every lane looks at one of 64 of those left
+__device__ __forceinline__ int request_of(const int32_t *cu, int B, int item, int mul, int div) {
+    int lo = 0, n = B;
+    const int lane = threadIdx.x & 63;
+    while (n > 1) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const bool le = i < n && first_item(cu, lo + i, mul, div) <= item;
+        const int k = max(1, __popcll(__ballot(le))) - 1;
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+inline size_t item_count(int B, int T, int mul, int div) { return (size_t) ((long long) T * mul / div) + B; }
+
+// over the lanes l, l ^ 16, l ^ 32, l ^ 48: the same bits in each
+__device__ __forceinline__ float max_quarters(float x) {
+    float2 r = swap16(x);
+    r = swap32(fmaxf(r.x, r.y));
+    return fmaxf(r.x, r.y);
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+    float2 r = swap16(x);
+    r = swap32(r.x + r.y);
+    return r.x + r.y;
+}
+
+}  // namespace fn

@@ -50,7 +50,8 @@ struct GdnChunk {
     float *o;                           // [T][nvh][dv]
     void *work;
     size_t work_bytes;
-    // the fused block (qkv set): conv1d + SiLU + L2-norm and gates in front, gated RMSNorm behind
+    // the fused block: conv1d + SiLU + L2-norm and gates in front, gated RMSNorm behind
+    bool block = false;
     int gate_act = 0, ring = 0;
     float eps = 0.0f;
     const int32_t *pos = nullptr;       // [B]
@@ -67,7 +68,7 @@ int kv4_unpack_launch(const Kv4Rows &p, hipStream_t st);
 size_t kv4_work_bytes(int B, int T, int nq, int nkv, int hd, int nsplit);
 int kv4_pick_nsplit(int B, int T, int nq, int nkv, int ctx);
 int kv4_attn_launch(const Kv4Attn &p, hipStream_t st);
-size_t gdn_chunk_work_bytes(int B, int T, int nkh, int nvh, bool block);
+size_t gdn_chunk_work_bytes(int B, int T, int nkh, int nvh);
 int gdn_chunk_launch(const GdnChunk &p, hipStream_t st);
 
 }  // namespace fn

@@ -41,6 +41,7 @@ SYMBOLS = (
     "fn_bench_gdn", "fn_bench_attn",
     "fn_page_plan_dev", "fn_page_release_dev", "fn_kv4_page_bytes", "fn_kv4_pack_dev", "fn_kv4_unpack_dev",
     "fn_attn_kv4_dev", "fn_attn_kv4_work_bytes", "fn_attn_kv4_nsplit",
+    "fn_gdn_core_chunk_dev", "fn_gdn_block_chunk_dev", "fn_gdn_chunk_work_bytes",
 )
 
 # the shapes fn_model_dims writes, in order (include/faie2fn.h section 6)
@@ -166,6 +167,10 @@ class FN:
         d.fn_attn_kv4_work_bytes.restype = sz
         d.fn_attn_kv4_work_bytes.argtypes = [i] * 6
         d.fn_attn_kv4_nsplit.argtypes = [i] * 5
+        d.fn_gdn_core_chunk_dev.argtypes = [i] * 7 + [VP] * 9 + [sz, VP]
+        d.fn_gdn_block_chunk_dev.argtypes = [i] * 9 + [VP] * 11 + [f, VP, VP, sz, VP]
+        d.fn_gdn_chunk_work_bytes.restype = sz
+        d.fn_gdn_chunk_work_bytes.argtypes = [i] * 4
 
     def check(self, rc):
         if rc != 0:
@@ -461,6 +466,22 @@ class FN:
         """The attention layer of a packed batch over the 4-bit paged cache."""
         self.check(self.d.fn_attn_kv4_dev(B, T, nq, nkv, hd, nrot, float(theta), float(eps), max_blocks, npages, past, cu,
                                           table, slot, seq, qg, k, v, wq, wk, cache, nsplit, work, work_bytes, og, stream))
+
+    def gdn_chunk_work_bytes(self, B, T, nkh, nvh):
+        return int(self.d.fn_gdn_chunk_work_bytes(B, T, nkh, nvh))
+
+    def gdn_core_chunk_dev(self, B, T, nkh, nvh, cu, q, k, v, beta, g, S, o, work, work_bytes, stream=0, dk=128, dv=128,
+                           head_map=0):
+        """The DeltaNet core over a packed batch of prompts."""
+        self.check(self.d.fn_gdn_core_chunk_dev(B, T, nkh, nvh, dk, dv, head_map, cu, q, k, v, beta, g, S, o, work,
+                                                work_bytes, stream))
+
+    def gdn_block_chunk_dev(self, B, T, nkh, nvh, ring, cu, pos, qkv, conv_w, conv_ring, ab, dt_bias, ssm_a, S, z,
+                            norm_w, out, work, work_bytes, stream=0, dk=128, dv=128, head_map=0, gate_act=0, eps=1e-6):
+        """The fused DeltaNet block over a packed batch of prompts."""
+        self.check(self.d.fn_gdn_block_chunk_dev(B, T, nkh, nvh, dk, dv, head_map, gate_act, ring, cu, pos, qkv, conv_w,
+                                                 conv_ring, ab, dt_bias, ssm_a, S, z, norm_w, float(eps), out, work,
+                                                 work_bytes, stream))
 
     # ---- path engine ----
     def path_init(self, B, nl, attn_every=4, nkh=16, nvh=32, nq=16, nkv=2, max_ctx=4096, head_map=0, gate_act=0,

@@ -330,6 +330,24 @@ int fn_attn_kv4_dev(int B, int T, int nq, int nkv, int hd, int nrot, float theta
 size_t fn_attn_kv4_work_bytes(int B, int T, int nq, int nkv, int hd, int nsplit);
 int fn_attn_kv4_nsplit(int B, int T, int nq, int nkv, int ctx);
 
+/* The DeltaNet core of fn_gdn_core_dev over a packed batch of prompts, 64 tokens at a time: q, k [T][nkh][dk],
+ * v [T][nvh][dv], beta, g [T][nvh], cu [B + 1], S [B][nvh][dk][dv] in/out, o [T][nvh][dv].  The state of a request without
+ * new tokens is left as it was.  An infinity or NaN in a request's inputs may reach all outputs of its value head from
+ * the start of the 64 tokens that hold it.  q, k, o and work 16-byte aligned; work: fn_gdn_chunk_work_bytes(B, T, nkh, nvh)
+ * bytes.  For one or a few tokens a request fn_gdn_core_dev and fn_gdn_block_dev are the faster calls. */
+int fn_gdn_core_chunk_dev(int B, int T, int nkh, int nvh, int dk, int dv, int head_map, const int32_t *cu, const float *q,
+                          const float *k, const float *v, const float *beta, const float *g, float *S, float *o,
+                          void *work, size_t work_bytes, void *stream);
+
+/* The fused block of fn_gdn_block_dev over a packed batch of prompts: qkv [T][C], ab [T][2 nvh], z, out [T][nvh dv];
+ * pos [B] tokens already seen; conv_ring [B][ring][C], ring a power of two >= 4, of which only the last three positions
+ * are read and written whatever the prompt's length.  conv_w, z, norm_w, out and work 16-byte aligned. */
+int fn_gdn_block_chunk_dev(int B, int T, int nkh, int nvh, int dk, int dv, int head_map, int gate_act, int ring,
+                           const int32_t *cu, const int32_t *pos, const float *qkv, const float *conv_w, float *conv_ring,
+                           const float *ab, const float *dt_bias, const float *ssm_a, float *S, const float *z,
+                           const float *norm_w, float eps, float *out, void *work, size_t work_bytes, void *stream);
+size_t fn_gdn_chunk_work_bytes(int B, int T, int nkh, int nvh);
+
 /* ======================================================================================================
  * 4. Path engine (new): the reference's Engine + layer_forward + forward (faie2fn.cu:1937-2031, 2370-2490) for
  *    this path only.  B sequences, nl layers; layer il is attention iff (il + 1) % attn_every == 0
