@@ -15,10 +15,11 @@ using namespace kv4;
 constexpr int MAXROT = 128;
 constexpr int NPART = 5;                               // fp6 parts of a query value
 constexpr int FRAG = 64 * 24;                          // a part's operand: 16 bytes, then 8 bytes a lane
-constexpr int QBLK = 2 * NPART * FRAG + 2 * 64 * 8;    // 16 query rows: [half][part] operands, [half] scales: 16 KiB
-static_assert(QBLK == 16384, "1 KiB a query row");
+constexpr int QBLK = 2 * NPART * FRAG + 2 * 64 * 8;    // 16 query rows: [half][part] operands, [half] scales
+constexpr int HSLOT = 3;                               // 8 query rows: columns 0..7 hold parts 0..2, 8..15 parts 3, 4, zero
+constexpr int HBLK = 2 * HSLOT * FRAG + 2 * 64 * 4;    // [half][slot] operands, [half] scales
+template <int RT> constexpr int item_bytes = RT == 8 ? HBLK : RT / 16 * QBLK;  // RT: query rows an item
 constexpr int WAVES = 4;
-constexpr int OS = 68;                                 // floats a row of the merge buffer (64 dims; rows 4 banks apart)
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
@@ -45,11 +46,43 @@ struct Kv4Args {
     double freq[MAXROT / 2];
 };
 
+// Sine and cosine in 64 bits of 0 <= x < 2^30: x less the nearest multiple of pi / 2, which is kept in two parts (the
+// first product is exact in the fused multiply-add), then the Taylor series to r^17, whose rest is below 2^-60 for
+// |r| <= pi / 4.
+__device__ __forceinline__ void sin_cos(double x, double &s, double &c) {
+    const double n = rint(x * 0.63661977236758134308);
+    double r = fma(-n, 1.5707963267948966192, x);
+    r = fma(-n, 6.123233995736766036e-17, r);
+    const double z = r * r;
+    double a = 2.8114572543455206e-15, b = 4.7794773323873853e-14;  // 1/17!, 1/16!
+    a = fma(a, z, -7.6471637318198164e-13);
+    b = fma(b, z, -1.1470745597729725e-11);
+    a = fma(a, z, 1.6059043836821613e-10);
+    b = fma(b, z, 2.0876756987868099e-09);
+    a = fma(a, z, -2.5052108385441719e-08);
+    b = fma(b, z, -2.7557319223985893e-07);
+    a = fma(a, z, 2.7557319223985893e-06);
+    b = fma(b, z, 2.4801587301587302e-05);
+    a = fma(a, z, -1.9841269841269841e-04);
+    b = fma(b, z, -1.3888888888888889e-03);
+    a = fma(a, z, 8.3333333333333333e-03);
+    b = fma(b, z, 4.1666666666666667e-02);
+    a = fma(a, z, -1.6666666666666667e-01);
+    b = fma(b, z, -0.5);
+    const double sr = fma(r * z, a, r), cr = fma(z, b, 1.0);
+    const int q = (int) n & 3;
+    s = q & 1 ? cr : sr;
+    c = q & 1 ? sr : cr;
+    if (q & 2) s = -s;
+    if (q == 1 || q == 2) c = -c;
+}
+
 // One token: sines and cosines of its position, its keys and values into their page, its queries as operands.
 template <int RT>
-__global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
-    __shared__ double cs[MAXROT / 2], sn[MAXROT / 2];
-    __shared__ double krow[WAVES][HD];
+__global__ void __launch_bounds__(256, 2) k_kv4_prep(const Kv4Args a) {
+    __shared__ double cs[MAXROT], sn[MAXROT];  // of each rotated dim; the sine with the sign that its pair's other value gets
+    __shared__ float cf[MAXROT], sf[MAXROT];
+    __shared__ double krow[WAVES][MAXROT];
     __shared__ float qrow[WAVES][8][MAXROT + 4];
     const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int total = min(a.cu[a.B], a.T);
@@ -63,7 +96,14 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
     if ((a.past[b] < 0 || P >= (long long) a.mb * PG) && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_POS);
     const int half = a.nrot / 2;
     // the angle in 64 bits: a float product is off by up to half a radian at a million tokens
-    if (threadIdx.x < half) sincos((double) P * a.freq[threadIdx.x], &sn[threadIdx.x], &cs[threadIdx.x]);
+    if (threadIdx.x < MAXROT) {
+        const int d = threadIdx.x;
+        double sv = 0.0, cv = 1.0;
+        if (d < a.nrot) sin_cos((double) P * a.freq[d < half ? d : d - half], sv, cv);
+        if (d < half) sv = -sv;
+        cs[d] = cv, sn[d] = sv;
+        cf[d] = (float) cv, sf[d] = (float) sv;
+    }
     __syncthreads();
     const int slot = a.slot[t];
     const bool put = slot >= 0 && slot / PG < a.npages;
@@ -87,18 +127,18 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
             for (int d = 1; d < 64; d <<= 1) ss += __shfl_xor(ss, d);
             const double r = 1.0 / sqrt(ss / HD + (double) a.eps);
             y[0] *= r * w.x, y[1] *= r * w.y, y[2] *= r * w.z, y[3] *= r * w.w;
+            if (4 * lane < a.nrot) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) krow[wave][4 * lane + i] = y[i];
+                for (int i = 0; i < 4; ++i) krow[wave][4 * lane + i] = y[i];
+            }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            if (4 * lane < a.nrot) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = 4 * lane + i;
-                if (d < a.nrot) {
-                    const int j = d < half ? d : d - half;
-                    const double x0 = krow[wave][j], x1 = krow[wave][j + half];
-                    y[i] = d < half ? x0 * cs[j] - x1 * sn[j] : x1 * cs[j] + x0 * sn[j];
+                for (int i = 0; i < 4; ++i) {
+                    const int d = 4 * lane + i, o = d < half ? d + half : d < a.nrot ? d - half : d;
+                    y[i] = y[i] * cs[d] + krow[wave][o] * sn[d];
                 }
             }
             store_row<true>(page, slot % PG, y, lane, a.status);
@@ -125,6 +165,7 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
         for (int i = 0; i < 8; ++i) {
             const float4 w = wsrc[i];
             x[4 * i] *= r * w.x, x[4 * i + 1] *= r * w.y, x[4 * i + 2] *= r * w.z, x[4 * i + 3] *= r * w.w;
+            if (i == 3) __builtin_amdgcn_sched_barrier(0);
         }
         if (32 * gi < a.nrot) {  // the rotated dims meet in the LDS
 #pragma unroll
@@ -136,13 +177,9 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
         if (32 * gi < a.nrot) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                const int d = 32 * gi + i;
-                if (d < a.nrot) {
-                    const int j = d < half ? d : d - half;
-                    const float x0 = qrow[wave][lane >> 3][j], x1 = qrow[wave][lane >> 3][j + half];
-                    const float c = (float) cs[j], s = (float) sn[j];
-                    x[i] = d < half ? x0 * c - x1 * s : x1 * c + x0 * s;
-                }
+                const int d = 32 * gi + i, o = d < half ? d + half : d < a.nrot ? d - half : d;
+                x[i] = fmaf(qrow[wave][lane >> 3][o], sf[d], x[i] * cf[d]);
+                if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // reads of eight at a time: 128 registers, four waves a SIMD
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -162,8 +199,8 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
         e0 = max(e0, EMIN);
         const int g = h / a.grp, row = (t - a.cu[b]) * a.grp + (h - g * a.grp);
         const int item = first_item(a.cu, b, a.grp, RT) + row / RT;
-        uint8_t *dst = a.Q + (((size_t) g * a.items + item) * (RT / 16) + row % RT / 16) * QBLK;
-        const int uh = gi >> 2, ln = (gi & 3) * 16 + row % 16;
+        uint8_t *dst = a.Q + ((size_t) g * a.items + item) * item_bytes<RT> + (RT == 8 ? 0 : row % RT / 16 * QBLK);
+        const int uh = gi >> 2, ln = (gi & 3) * 16 + row % (RT == 8 ? 8 : 16);
         const bool st = on && item < a.items;
         v16f lo, hi;
 #pragma unroll
@@ -177,8 +214,10 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
             // operands are kept in use past each of them)
             asm volatile("" ::"v"(lo), "v"(hi), "v"(sc), "v"(part));
             if (st) {
-                *reinterpret_cast<v4u *>(dst + (uh * NPART + p) * FRAG + ln * 16) = v4u{part[0], part[1], part[2], part[3]};
-                *reinterpret_cast<v2u *>(dst + (uh * NPART + p) * FRAG + 1024 + ln * 8) = v2u{part[4], part[5]};
+                uint8_t *f = dst + (RT == 8 ? uh * HSLOT + p % HSLOT : uh * NPART + p) * FRAG;
+                const int l = ln + (RT == 8 && p >= HSLOT ? 8 : 0);
+                *reinterpret_cast<v4u *>(f + l * 16) = v4u{part[0], part[1], part[2], part[3]};
+                *reinterpret_cast<v2u *>(f + 1024 + l * 8) = v2u{part[4], part[5]};
             }
             if (p + 1 < NPART) {
                 const v32f back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(part, sc);
@@ -192,7 +231,18 @@ __global__ void __launch_bounds__(256) k_kv4_prep(const Kv4Args a) {
         const uint32_t s0 = e0 + 127;
         const v2u sc = bad ? v2u{~0u, ~0u}
                            : v2u{s0 | (s0 - 4) << 8 | (s0 - 9) << 16 | (s0 - 14) << 24, s0 - 19};
-        if (st) *reinterpret_cast<v2u *>(dst + 2 * NPART * FRAG + uh * 512 + ln * 8) = sc;
+        if (RT == 8) {
+            if (st) {
+                uint8_t *f = dst + (uh * HSLOT + 2) * FRAG;
+                *reinterpret_cast<v4u *>(f + (ln + 8) * 16) = v4u{0, 0, 0, 0};
+                *reinterpret_cast<v2u *>(f + 1024 + (ln + 8) * 8) = v2u{0, 0};
+                uint32_t *d = reinterpret_cast<uint32_t *>(dst + 2 * HSLOT * FRAG + uh * 256) + ln;
+                d[0] = sc[0];
+                d[8] = sc[0] >> 24 | (sc[1] & 0xff) << 8;  // parts 3, 4
+            }
+        } else if (st) {
+            *reinterpret_cast<v2u *>(dst + 2 * NPART * FRAG + uh * 512 + ln * 8) = sc;
+        }
     }
 }
 
@@ -211,22 +261,88 @@ constexpr float SM_SCALE = 0.0625f * 1.4426950408889634f;  // 1 / sqrt(HD), and 
 constexpr float SLACK = 8.0f * 16.0f;                      // growth of a row's largest raw score that moves its reference
 constexpr float PUP = 16.0f;                               // probabilities times 2^16: the parts of the least ones stay normal
 
-struct KvBlock {  // 32 keys of one head in registers
+// A 32-key block of one head in 49 registers.  A wave holds two; what it has used up it requests of the next block but one
+// at once (K behind the scores, V behind each pair of its groups), so that about one and a half blocks are in flight.
+struct KvBlock {
     v4u k[2][2];  // [16-key block][half of the row]
     uint32_t ks;
     v4u v[4], vs[4];
+    __device__ __forceinline__ void load_k(const uint8_t *p, int kk, int lane) {
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                k[hb][u] = *reinterpret_cast<const v4u *>(p + kk * 4096 + (hb * 2 + u) * 1024 + lane * 16);
+        ks = *reinterpret_cast<const uint32_t *>(p + KS + kk * 256 + lane * 4);
+    }
+    __device__ __forceinline__ void load_v(int i, const uint8_t *p, int kk, int lane) {
+        v[i] = *reinterpret_cast<const v4u *>(p + VC + kk * 4096 + i * 1024 + lane * 16);
+        vs[i] = *reinterpret_cast<const v4u *>(p + VS + kk * 256 + i * 16 + (lane >> 4) * 64);
+    }
+    // values of the lane's dims 32 t + 2 (l % 16), + 1 of its eight keys
+    __device__ __forceinline__ void values(int t, uint32_t (&x)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t w = v[t / 2][t % 2 * 2 + j / 4], s4 = vs[t / 2][t % 2 * 2 + j / 4];
+            // the instruction takes the scale from bits 30:23 of a float and looks at no other
+            const float s = __uint_as_float(j % 4 == 3 ? s4 >> 1 : s4 << (23 - 8 * (j % 4)));
+            const auto cv = [&](auto sel) {
+                return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, decltype(sel)::value));
+            };
+            x[j] = j % 4 == 0   ? cv(std::integral_constant<int, 0>{})
+                   : j % 4 == 1 ? cv(std::integral_constant<int, 1>{})
+                   : j % 4 == 2 ? cv(std::integral_constant<int, 2>{})
+                                : cv(std::integral_constant<int, 3>{});
+        }
+    }
 };
 
-// grid (nsplit, nkv, items), 256 threads: the RT = 16 NRB rows of an item against the keys of a split; the waves take
+// The state of one row (the lane's column) of an online softmax.  MASK: keys from lim on count for nothing.
+struct Softmax {
+    float m = -INFINITY, l = 0.0f;
+    // eight raw scores (key + 16 (i / 4) + i % 4) -> probabilities 2^PUP p; returns the factor of what was summed before
+    template <bool MASK> __device__ __forceinline__ float step(const float (&s)[8], float (&p)[8], int key, int lim) {
+        float sc[8], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sc[i] = !MASK || key + 16 * (i / 4) + i % 4 < lim ? s[i] : -INFINITY;
+            mx = fmaxf(mx, sc[i]);
+        }
+        mx = max_quarters(mx);
+        const bool first = m == -INFINITY, moved = !first && mx > m + SLACK;
+        const float mn = first || moved ? mx : m;
+        const float corr = moved ? __builtin_amdgcn_exp2f((m - mn) * SM_SCALE) : 1.0f;
+        float ps = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i] - mn, SM_SCALE, PUP));
+            if (MASK && sc[i] == -INFINITY) p[i] = 0.0f;
+            ps += p[i];
+        }
+        l = fmaf(l, corr, ps);
+        m = mn;
+        return corr;
+    }
+};
+
+// grid (nsplit, nkv, items), 256 threads: the RT rows of an item (8, 16 or 32) against the keys of a split; the waves take
 // 32-key blocks in turn, each with its own softmax state, and meet at the end.
-template <int NRB>
-__global__ void __launch_bounds__(WAVES * 64) k_attn_kv4(const Kv4Args a) {
-    constexpr int RT = 16 * NRB;
-    constexpr int QB = NRB * QBLK, MB = WAVES * RT * OS * 4;
+// Eight rows (a decode step of up to 8 query heads a kv head) use both halves of the products' 16 columns.  Scores:
+// columns 0..7 take parts 0..2 of the queries and 8..15 parts 3, 4, so three products do for five, and a rotation by
+// eight lanes adds the halves.  P.V: the conversion leaves dims 2m, 2m + 1 of a key in one register, which as it stands
+// is two contraction slots; the columns 0..7 hold a probability in the first of them and 0 in the second, which gives
+// the even dims, and 8..15 the other way round.  So nothing is permuted and the sums take half the registers.
+template <int RT>
+__global__ void __launch_bounds__(WAVES * 64, RT == 32 ? 1 : RT == 16 ? 2 : 3) k_attn_kv4(const Kv4Args a) {
+    constexpr bool HALF = RT == 8;
+    constexpr int NRB = HALF ? 1 : RT / 16, NT = HALF ? 8 : 16;      // row blocks, output tiles a row block
+    constexpr int NB = 1;                                 // key blocks in registers
+    constexpr int DC = HALF ? 256 : 64, MS = DC + 4;                 // dims merged at a time, floats a row of the merge
+    constexpr int QB = item_bytes<RT>, MB = WAVES * RT * MS * 4;
     __shared__ __align__(16) uint8_t lds[QB > MB ? QB : MB];
     __shared__ float wm[WAVES][RT], wl[WAVES][RT];
     const int sp = blockIdx.x, g = blockIdx.y, item = a.items - 1 - (int) blockIdx.z;  // the longest rows first
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int b = request_of(a.cu, a.B, item, a.grp, RT);
     const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r0 = (item - first_item(a.cu, b, a.grp, RT)) * RT;
     const int rows = n * a.grp;
@@ -236,87 +352,105 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_kv4(const Kv4Args a) {
     const int kvalid = visible(n - 1), kmax = visible((min(r0 + RT, rows) - 1) / a.grp);
     const int tiles = (kmax + PG - 1) / PG, per = (tiles + a.nsplit - 1) / a.nsplit;
     const int k0 = min(sp * per, tiles) * PG, k1 = min(min((sp + 1) * per, tiles) * PG, kmax);
+    const int all = min(visible(r0 / a.grp), k1);  // keys that every row of the item sees
 
+    // through the scalar cache: a vector load's wait would wait for every key block in flight, too
+    typedef const __attribute__((address_space(4))) int32_t *scalar_i32;
+    const scalar_i32 table = (scalar_i32) (uintptr_t) (a.table + (size_t) b * a.mb);
+    const size_t stride = (size_t) a.nkv * HEAD_BYTES;
+    const uint8_t *cache = a.cache + (size_t) g * HEAD_BYTES;
+    auto page_of = [&](int kb) { return kb * 32 < k1 ? table[kb >> 1] : 0; };
+    auto ok = [&](int page) { return page >= 0 && page < a.npages; };
+    auto base_of = [&](int page) { return cache + (ok(page) ? page : 0) * stride; };  // in bounds; the block is passed over
+    int kb = k0 / 32 + wave;
+    int page[NB + 1];  // of this block and the next ones
+#pragma unroll
+    for (int i = 0; i <= NB; ++i) page[i] = page_of(kb + i * WAVES);
+    KvBlock x[NB];
+    auto load_all = [&](KvBlock &y, int at, int pg) __attribute__((always_inline)) {
+        const uint8_t *p = base_of(pg);
+        y.load_k(p, at & 1, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y.load_v(i, p, at & 1, lane);
+    };
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+        if ((kb + i * WAVES) * 32 < k1) load_all(x[i], kb + i * WAVES, page[i]);
     // the item's query operands into the LDS
-    const v4u *Q = reinterpret_cast<const v4u *>(a.Q + ((size_t) g * a.items + item) * NRB * QBLK);
+    const v4u *Q = reinterpret_cast<const v4u *>(a.Q + ((size_t) g * a.items + item) * item_bytes<RT>);
     for (int i = threadIdx.x; i < QB / 16; i += WAVES * 64) reinterpret_cast<v4u *>(lds)[i] = Q[i];
     __syncthreads();
-    int lim[NRB];
+    uint32_t hs[2];
     v2u qs[NRB][2];
 #pragma unroll
-    for (int j = 0; j < NRB; ++j) {
-        lim[j] = min(visible(min((r0 + 16 * j + (lane & 15)) / a.grp, n - 1)), k1);
+    for (int u = 0; u < 2; ++u) {
+        if (HALF) hs[u] = *reinterpret_cast<const uint32_t *>(lds + 2 * HSLOT * FRAG + u * 256 + lane * 4);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-            qs[j][u] = *reinterpret_cast<const v2u *>(lds + j * QBLK + 2 * NPART * FRAG + u * 512 + lane * 8);
+        for (int j = 0; j < NRB; ++j)
+            if (!HALF) qs[j][u] = *reinterpret_cast<const v2u *>(lds + j * QBLK + 2 * NPART * FRAG + u * 512 + lane * 8);
     }
-    v4f o[NRB][16];
-    float m[NRB], l[NRB];
-#pragma unroll
-    for (int j = 0; j < NRB; ++j) {
-        m[j] = -INFINITY;
-        l[j] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) o[j][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const int32_t *table = a.table + (size_t) b * a.mb;
-    auto page_of = [&](int kb) { return kb * 32 < k1 ? table[kb >> 1] : 0; };
-    auto load = [&](int kb, int page, KvBlock &x) {
-        if (page < 0 || page >= a.npages) page = 0;  // in bounds; the block is skipped
-        const uint8_t *p = a.cache + ((size_t) page * a.nkv + g) * HEAD_BYTES;
-        const int kk = kb & 1;
-#pragma unroll
-        for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                x.k[hb][u] = *reinterpret_cast<const v4u *>(p + (((kk * 2 + hb) * 2 + u) * 64 + lane) * 16);
-        x.ks = *reinterpret_cast<const uint32_t *>(p + KS + (kk * 64 + lane) * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x.v[i] = *reinterpret_cast<const v4u *>(p + VC + ((kk * 4 + i) * 64 + lane) * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            x.vs[i] = *reinterpret_cast<const v4u *>(p + VS + (kk * 4 + (lane >> 4)) * 64 + i * 16);
+    auto operand = [&](int at) __attribute__((always_inline)) {
+        const v4u qa = *reinterpret_cast<const v4u *>(lds + at + lane * 16);
+        const v2u qb = *reinterpret_cast<const v2u *>(lds + at + 1024 + lane * 8);
+        return v6u{qa[0], qa[1], qa[2], qa[3], qb[0], qb[1]};
     };
-    int kb = k0 / 32 + wave;
-    int page = page_of(kb), next_page = page_of(kb + WAVES);
-    KvBlock cur, nxt;
-    if (kb * 32 < k1) load(kb, page, cur);
-    for (; kb * 32 < k1; kb += WAVES) {
-        const int here = page;
-        page = next_page;
-        next_page = page_of(kb + 2 * WAVES);
-        load((kb + WAVES) * 32 < k1 ? kb + WAVES : kb, (kb + WAVES) * 32 < k1 ? page : here, nxt);
-        if (here < 0 || here >= a.npages) {
-            if (lane == 0) atomicOr(a.status, FN_STATUS_PAGE);
-            cur = nxt;
-            continue;
-        }
-        if (kb * 32 + 32 > kvalid) {  // rows of the page that hold no token: their value scales may be anything
-            const int base = kb * 32 + 4 * (lane >> 4);
-            uint32_t keep[2] = {0, 0};
+    int lim[NRB];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) keep[j / 4] |= base + 16 * (j / 4) + j % 4 < kvalid ? 0xffu << (8 * (j % 4)) : 0u;
+    for (int j = 0; j < NRB; ++j)
+        lim[j] = min(visible(min((r0 + 16 * j + (lane & (HALF ? 7 : 15))) / a.grp, n - 1)), k1);
+    v4f o[NRB][NT];
+    Softmax sm[NRB];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) cur.vs[i] &= v4u{keep[0], keep[1], keep[0], keep[1]};
-        }
-        // scores
-        v4f S[2][NRB];
-        {
+    for (int j = 0; j < NRB; ++j)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[j][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    auto block = [&](KvBlock &x) __attribute__((always_inline)) {
+        // what takes the place of this block: the NB-th after it (at the end, this one again)
+        const bool more = (kb + NB * WAVES) * 32 < k1;
+        const int here = page[0], kn = more ? kb + NB * WAVES : kb, pn = more ? page[NB] : here;
+        const uint8_t *p = base_of(pn);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) page[i] = page[i + 1];
+        page[NB] = page_of(kb + (NB + 1) * WAVES);
+        const bool in = ok(here);  // a block outside the cache counts for nothing
+        if (!in && lane == 0) atomicOr(a.status, FN_STATUS_PAGE);
+        // scores, in two sums: what the first part of the queries gives, and the small rest
+        float S[NRB][8];
+        const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (HALF) {
+            v4f big[2] = {zero, zero}, small[2] = {zero, zero};
+#define FN_KV4_SLOT(U, P)                                                                              \
+    do {                                                                                              \
+        const v6u q = operand(((U) * HSLOT + (P)) * FRAG);                                             \
+        v4f(&acc)[2] = (P) == 0 ? big : small;                                                         \
+        acc[0] = mma_k<(U), (P)>(x.k[0][U], (int) x.ks, q, (int) hs[U], acc[0]);                       \
+        acc[1] = mma_k<2 + (U), (P)>(x.k[1][U], (int) x.ks, q, (int) hs[U], acc[1]);                   \
+    } while (0)
+            FN_KV4_SLOT(0, 1);
+            FN_KV4_SLOT(0, 0);
+            FN_KV4_SLOT(0, 2);
+            FN_KV4_SLOT(1, 0);
+            FN_KV4_SLOT(1, 1);
+            FN_KV4_SLOT(1, 2);
+#undef FN_KV4_SLOT
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float s = big[i / 4][i % 4] + small[i / 4][i % 4];
+                S[0][i] = s + dpp_ror<8>(s);
+            }
+        } else {
             v4f big[2][NRB], small[2][NRB];
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
-                for (int j = 0; j < NRB; ++j) big[hb][j] = small[hb][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int j = 0; j < NRB; ++j) big[hb][j] = small[hb][j] = zero;
 #define FN_KV4_PART(U, P)                                                                                            \
     do {                                                                                                            \
         _Pragma("unroll") for (int j = 0; j < NRB; ++j) {                                                            \
-            const uint8_t *f = lds + j * QBLK + ((U) * NPART + (P)) * FRAG;                                          \
-            const v4u qa = *reinterpret_cast<const v4u *>(f + lane * 16);                                            \
-            const v2u qb = *reinterpret_cast<const v2u *>(f + 1024 + lane * 8);                                      \
-            const v6u q = {qa[0], qa[1], qa[2], qa[3], qb[0], qb[1]};                                                \
+            const v6u q = operand(j * QBLK + ((U) * NPART + (P)) * FRAG);                                            \
             v4f(&acc)[2][NRB] = (P) == 0 ? big : small;                                                              \
-            acc[0][j] = mma_k<(U), (P) % 4>(cur.k[0][U], (int) cur.ks, q, (int) qs[j][U][(P) / 4], acc[0][j]);       \
-            acc[1][j] = mma_k<2 + (U), (P) % 4>(cur.k[1][U], (int) cur.ks, q, (int) qs[j][U][(P) / 4], acc[1][j]);   \
+            acc[0][j] = mma_k<(U), (P) % 4>(x.k[0][U], (int) x.ks, q, (int) qs[j][U][(P) / 4], acc[0][j]);           \
+            acc[1][j] = mma_k<2 + (U), (P) % 4>(x.k[1][U], (int) x.ks, q, (int) qs[j][U][(P) / 4], acc[1][j]);       \
         }                                                                                                           \
     } while (0)
             FN_KV4_PART(0, 0);
@@ -331,113 +465,161 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_kv4(const Kv4Args a) {
             FN_KV4_PART(1, 4);
 #undef FN_KV4_PART
 #pragma unroll
-            for (int hb = 0; hb < 2; ++hb)
+            for (int j = 0; j < NRB; ++j)
 #pragma unroll
-                for (int j = 0; j < NRB; ++j) S[hb][j] = big[hb][j] + small[hb][j];
+                for (int i = 0; i < 8; ++i) S[j][i] = big[i / 4][j][i % 4] + small[i / 4][j][i % 4];
         }
-        // online softmax of the lane's row (lane % 16) over the 32 keys; the probabilities in three bf16 parts
-        v4u P[NRB][3];
-        float corr[NRB];
-        bool rescale = false;
+        x.load_k(p, kn & 1, lane);
+        if (!in || kb * 32 + 32 > kvalid) {  // rows of the page that hold no token: their value scales may be anything
+            const int at = kb * 32 + 4 * (lane >> 4), end = in ? kvalid : 0;
+            uint32_t keep[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) keep[j / 4] |= at + 16 * (j / 4) + j % 4 < end ? 0xffu << (8 * (j % 4)) : 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.vs[i] &= v4u{keep[0], keep[1], keep[0], keep[1]};
+        }
+        float pr[NRB][8], corr[NRB];
+        bool moved = false;
         const int key = kb * 32 + 4 * (lane >> 4);
 #pragma unroll
         for (int j = 0; j < NRB; ++j) {
-            float sc[8], mx = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                sc[i] = key + 16 * (i / 4) + i % 4 < lim[j] ? S[i / 4][j][i % 4] : -INFINITY;
-                mx = fmaxf(mx, sc[i]);
-            }
-            mx = max_quarters(mx);
-            const bool first = m[j] == -INFINITY, moved = !first && mx > m[j] + SLACK;
-            const float mn = first || moved ? mx : m[j];
-            corr[j] = moved ? __builtin_amdgcn_exp2f((m[j] - mn) * SM_SCALE) : 1.0f;
-            rescale |= moved;
-            float ps = 0.0f;
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                p[i] = sc[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(sc[i] - mn, SM_SCALE, PUP));
-                ps += p[i];
-            }
-            l[j] = fmaf(l[j], corr[j], ps);
-            m[j] = mn;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x = p[2 * i], y = p[2 * i + 1];
-#pragma unroll
-                for (int q = 0; q < 3; ++q) {
-                    const uint32_t h = bf16_pair(x, y);
-                    P[j][q][i] = h;
-                    x -= __uint_as_float(h << 16);
-                    y -= __uint_as_float(h & 0xffff0000u);
-                }
-            }
+            corr[j] = in && kb * 32 + 32 <= all ? sm[j].template step<false>(S[j], pr[j], key, lim[j])
+                                                : sm[j].template step<true>(S[j], pr[j], key, in ? lim[j] : 0);
+            moved |= corr[j] != 1.0f;
         }
-        if (__ballot(rescale)) {
+        if (__ballot(moved)) {
 #pragma unroll
             for (int j = 0; j < NRB; ++j)
 #pragma unroll
-                for (int t = 0; t < 16; ++t) o[j][t] *= corr[j];
+                for (int t = 0; t < NT; ++t) o[j][t] *= corr[j];
         }
-        // o += V^T P^T, 32 dims at a time: one conversion gives two dims of a key, a permute two keys of a dim
+        // o += V^T P^T, 32 dims at a time, the probabilities in three bf16 parts
+        if constexpr (HALF) {
+            v4u P[2][3];  // [16-key block][part]; parts by truncation (8 bits each: exact), in the half of the register that
+                          // the column takes
+            const int sh = lane & 8 ? 0 : 16;
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            uint32_t pr[8];
+            for (int i = 0; i < 8; ++i) {
+                float f = pr[0][i];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t w = cur.v[t / 2][t % 2 * 2 + j / 4], s4 = cur.vs[t / 2][t % 2 * 2 + j / 4];
-                // the instruction takes the scale from bits 30:23 of a float and looks at no other
-                const float s = __uint_as_float(j % 4 == 3 ? s4 >> 1 : s4 << (23 - 8 * (j % 4)));
-                const auto cv = [&](auto sel) {
-                    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, decltype(sel)::value));
-                };
-                pr[j] = j % 4 == 0   ? cv(std::integral_constant<int, 0>{})
-                        : j % 4 == 1 ? cv(std::integral_constant<int, 1>{})
-                        : j % 4 == 2 ? cv(std::integral_constant<int, 2>{})
-                                     : cv(std::integral_constant<int, 3>{});
-            }
-            v4u even, odd;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                even[i] = __builtin_amdgcn_perm(pr[2 * i + 1], pr[2 * i], 0x05040100u);
-                odd[i] = __builtin_amdgcn_perm(pr[2 * i + 1], pr[2 * i], 0x07060302u);
-            }
-#pragma unroll
-            for (int q = 2; q >= 0; --q)
-#pragma unroll
-                for (int j = 0; j < NRB; ++j) {
-                    o[j][2 * t] = mma_v(even, P[j][q], o[j][2 * t]);
-                    o[j][2 * t + 1] = mma_v(odd, P[j][q], o[j][2 * t + 1]);
+                for (int q = 0; q < 3; ++q) {
+                    const uint32_t h = __float_as_uint(f) & 0xffff0000u;
+                    P[i / 4][q][i % 4] = h >> sh;
+                    f -= __uint_as_float(h);
                 }
+            }
+            uint32_t w[2][8];
+            x.values(0, w[0]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {  // the next 32 dims are converted between the products
+                if (t < 7) x.values(t + 1, w[(t + 1) & 1]);
+                if (t % 2 == 0 && t < 6) x.load_v(t / 2, p, kn & 1, lane);
+                if (t == 7) x.load_v(3, p, kn & 1, lane);
+#pragma unroll
+                for (int q = 2; q >= 0; --q)
+#pragma unroll
+                    for (int hb = 0; hb < 2; ++hb) {
+                        const uint32_t *y = w[t & 1] + 4 * hb;
+                        o[0][t] = mma_v(v4u{y[0], y[1], y[2], y[3]}, P[hb][q], o[0][t]);
+                    }
+#pragma unroll
+                for (int i = 0; i < 6; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            v4u P[NRB][3];
+#pragma unroll
+            for (int j = 0; j < NRB; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f = pr[j][2 * i], h = pr[j][2 * i + 1];
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        const uint32_t w = bf16_pair(f, h);
+                        P[j][q][i] = w;
+                        f -= __uint_as_float(w << 16);
+                        h -= __uint_as_float(w & 0xffff0000u);
+                    }
+                }
+            v4u ve[2], vo[2];  // one dim of two keys
+            auto values = [&](int t) __attribute__((always_inline)) {
+                uint32_t w[8];
+                x.values(t, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ve[t & 1][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+                    vo[t & 1][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+                }
+            };
+            values(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                if (t < 7) values(t + 1);
+                if (t % 2 == 0 && t < 6) x.load_v(t / 2, p, kn & 1, lane);
+                if (t == 7) x.load_v(3, p, kn & 1, lane);
+#pragma unroll
+                for (int q = 2; q >= 0; --q)
+#pragma unroll
+                    for (int j = 0; j < NRB; ++j) {
+                        o[j][2 * t] = mma_v(ve[t & 1], P[j][q], o[j][2 * t]);
+                        o[j][2 * t + 1] = mma_v(vo[t & 1], P[j][q], o[j][2 * t + 1]);
+                    }
+#pragma unroll
+                for (int i = 0; i < 6 * NRB; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x2, 4 / NRB, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        cur = nxt;
+    };
+    while (kb * 32 < k1) {
+        block(x[0]);
+        kb += WAVES;
+        if (NB > 1) {
+            if (kb * 32 >= k1) break;
+            block(x[NB - 1]);
+            kb += WAVES;
+        }
     }
-    // the waves meet: reference of every row, then the sums, 64 dims at a time
+    // the waves meet: reference of every row, then the sums, DC dims at a time
 #pragma unroll
     for (int j = 0; j < NRB; ++j) {
-        const float ls = sum_quarters(l[j]);
-        if (lane < 16) {
-            wm[wave][16 * j + lane] = m[j];
+        const float ls = sum_quarters(sm[j].l);
+        if (lane < (HALF ? 8 : 16)) {
+            wm[wave][16 * j + lane] = sm[j].m;
             wl[wave][16 * j + lane] = ls;
         }
     }
     float *mo = reinterpret_cast<float *>(lds);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        __syncthreads();  // the query operands, or the last 64 dims, have been read
+    for (int c = 0; c < HD / DC; ++c) {
+        __syncthreads();  // the query operands, or the last dims, have been read
+        if constexpr (HALF) {
+            float *d = mo + (wave * RT + (lane & 7)) * MS + 8 * (lane >> 4) + ((lane >> 3) & 1);
 #pragma unroll
-        for (int j = 0; j < NRB; ++j)
+            for (int t = 0; t < 8; ++t)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {  // the lane's row, dims 8 (lane / 16) .. + 7 of the group
-                float *d = mo + (wave * RT + 16 * j + (lane & 15)) * OS + 32 * t + 8 * (lane >> 4);
-                const v4f e = o[j][4 * c + 2 * t], f = o[j][4 * c + 2 * t + 1];
-                *reinterpret_cast<float4 *>(d) = make_float4(e[0], f[0], e[1], f[1]);
-                *reinterpret_cast<float4 *>(d + 4) = make_float4(e[2], f[2], e[3], f[3]);
-            }
+                for (int i = 0; i < 4; ++i) d[32 * t + 2 * i] = o[0][t][i];
+        } else {
+#pragma unroll
+            for (int j = 0; j < NRB; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {  // the lane's row, dims 8 (lane / 16) .. + 7 of the group
+                    float *d = mo + (wave * RT + 16 * j + (lane & 15)) * MS + 32 * t + 8 * (lane >> 4);
+                    const v4f e = o[j][4 * c + 2 * t], f = o[j][4 * c + 2 * t + 1];
+                    *reinterpret_cast<float4 *>(d) = make_float4(e[0], f[0], e[1], f[1]);
+                    *reinterpret_cast<float4 *>(d + 4) = make_float4(e[2], f[2], e[3], f[3]);
+                }
+        }
         __syncthreads();
-        for (int i = threadIdx.x; i < RT * 16; i += WAVES * 64) {
-            const int row = i >> 4, r = r0 + row, d = (i & 15) * 4;
+        for (int i = threadIdx.x; i < RT * DC / 4; i += WAVES * 64) {
+            const int row = i / (DC / 4), r = r0 + row, d = i % (DC / 4) * 4;
             if (r >= rows) continue;
             float M = wm[0][row];
 #pragma unroll
@@ -449,19 +631,19 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_kv4(const Kv4Args a) {
                 const float mw = wm[w][row];
                 const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - M) * SM_SCALE);
                 L = fmaf(wl[w][row], f, L);
-                s = add_scaled(s, *reinterpret_cast<const float4 *>(mo + (w * RT + row) * OS + d), f);
+                s = add_scaled(s, *reinterpret_cast<const float4 *>(mo + (w * RT + row) * MS + d), f);
             }
             if (a.nsplit == 1) {
                 const int t = r / a.grp;
                 const size_t at = (size_t) (c0 + t) * a.nq + g * a.grp + (r - t * a.grp);
-                const float4 z = *reinterpret_cast<const float4 *>(a.qg + (at * 2 + 1) * HD + 64 * c + d);
+                const float4 z = *reinterpret_cast<const float4 *>(a.qg + (at * 2 + 1) * HD + DC * c + d);
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees no key: zeros
-                *reinterpret_cast<float4 *>(a.og + at * HD + 64 * c + d) =
+                *reinterpret_cast<float4 *>(a.og + at * HD + DC * c + d) =
                     make_float4(s.x * inv * sigmoidf_(z.x), s.y * inv * sigmoidf_(z.y), s.z * inv * sigmoidf_(z.z),
                                 s.w * inv * sigmoidf_(z.w));
             } else {
                 const size_t at = (((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + row;
-                *reinterpret_cast<float4 *>(a.part_o + at * HD + 64 * c + d) = s;
+                *reinterpret_cast<float4 *>(a.part_o + at * HD + DC * c + d) = s;
                 if (c == 0 && d == 0) {
                     a.part_ml[2 * at] = M;
                     a.part_ml[2 * at + 1] = L;
@@ -471,26 +653,38 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_kv4(const Kv4Args a) {
     }
 }
 
-// grid (items RT / 4, nkv), a wave a row, lane = 4 dims: the splits of a row joined, and the gate
+// grid (items RT, nkv), four waves a row, lane = 4 dims: the splits of a row joined, and the gate
 template <int RT>
 __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
-    const int item = blockIdx.x / (RT / 4), g = blockIdx.y, lane = threadIdx.x & 63;
-    const int row = blockIdx.x % (RT / 4) * 4 + (threadIdx.x >> 6);
+    __shared__ float4 part[WAVES][HD / 4];
+    __shared__ float pl[WAVES];
+    const int item = blockIdx.x / RT, g = blockIdx.y, row = blockIdx.x % RT, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = request_of(a.cu, a.B, item, a.grp, RT);
     const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r = (item - first_item(a.cu, b, a.grp, RT)) * RT + row;
     if (c0 < 0 || r < 0 || r >= n * a.grp) return;
     const size_t at0 = ((size_t) item * a.nkv + g) * a.nsplit * RT + row;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml);
     float M = -INFINITY;
-    for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, a.part_ml[2 * (at0 + (size_t) s * RT)]);
+    for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, ml[at0 + (size_t) s * RT].x);
     M = wave_max(M);
     float L = 0.0f;
     float4 o = f4(0.0f);
-    for (int s = 0; s < a.nsplit; ++s) {
+#pragma unroll 4
+    for (int s = wave; s < a.nsplit; s += WAVES) {
         const size_t at = at0 + (size_t) s * RT;
-        const float ms = a.part_ml[2 * at], ls = a.part_ml[2 * at + 1];
-        const float f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ms - M) * SM_SCALE);
-        L = fmaf(ls, f, L);
+        const float2 x = ml[at];
+        const float f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x.x - M) * SM_SCALE);
+        L = fmaf(x.y, f, L);
         o = add_scaled(o, reinterpret_cast<const float4 *>(a.part_o + at * HD)[lane], f);
+    }
+    part[wave][lane] = o;
+    if (lane == 0) pl[wave] = L;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+        o = add_scaled(o, part[w][lane], 1.0f);
+        L += pl[w];
     }
     const int t = r / a.grp;
     const size_t at = (size_t) (c0 + t) * a.nq + g * a.grp + (r - t * a.grp);
@@ -500,20 +694,30 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
         o.x * inv * sigmoidf_(z.x), o.y * inv * sigmoidf_(z.y), o.z * inv * sigmoidf_(z.z), o.w * inv * sigmoidf_(z.w));
 }
 
-// 16-row blocks an item: one where the requests have few rows (decode), two otherwise
-int row_blocks(int B, int T, int grp) { return (long long) T * grp <= 16ll * B ? 1 : 2; }
+template <int RT> void launch(const Kv4Args &a, hipStream_t st) {
+    hipLaunchKernelGGL(k_kv4_prep<RT>, dim3(a.T), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_attn_kv4<RT>, dim3(a.nsplit, a.nkv, a.items), dim3(WAVES * 64), 0, st, a);
+    if (a.nsplit > 1) hipLaunchKernelGGL(k_kv4_combine<RT>, dim3(a.items * RT, a.nkv), dim3(256), 0, st, a);
+}
+
+// Query rows an item: what an average request has, up to 32.
+int item_rows(int B, int T, int grp) {
+    const long long rows = (long long) T * grp;
+    return rows <= 8ll * B ? 8 : rows <= 16ll * B ? 16 : 32;
+}
+size_t query_bytes(int rt) { return rt == 8 ? HBLK : rt * 1024; }
 
 }  // namespace
 
 size_t kv4_work_bytes(int B, int T, int nq, int nkv, int hd, int nsplit) {
-    const int grp = nq / nkv, rt = 16 * row_blocks(B, T, grp);
-    const size_t rows = item_count(B, T, grp, rt) * nkv * rt;
-    return rows * 1024 + (nsplit > 1 ? rows * nsplit * (HD + 2) * sizeof(float) : 0);
+    const int grp = nq / nkv, rt = item_rows(B, T, grp);
+    const size_t n = item_count(B, T, grp, rt) * nkv;
+    return n * query_bytes(rt) + (nsplit > 1 ? n * rt * nsplit * (HD + 2) * sizeof(float) : 0);
 }
 
 int kv4_pick_nsplit(int B, int T, int nq, int nkv, int ctx) {
-    const int grp = nq / nkv;
-    const long long groups = (long long) item_count(B, T, grp, 16 * row_blocks(B, T, grp)) * nkv;
+    const int grp = nq / nkv, rt = item_rows(B, T, grp);
+    const long long groups = std::max<long long>(B, ((long long) T * grp + rt - 1) / rt) * nkv;
     const int most = std::max(1, (ctx + 127) / 128);  // a 32-key block for each wave
     const long long want = std::max(1ll, 2ll * device_cus() / groups);
     return (int) std::min<long long>(want, most);
@@ -524,6 +728,7 @@ int kv4_attn_launch(const Kv4Attn &p, hipStream_t st) {
     if (p.hd != HD) FN_FAIL("attn_kv4: only head_dim 256 is built");
     if (p.nq % p.nkv) FN_FAIL("attn_kv4: nq must be a multiple of nkv");
     if (p.nrot < 0 || p.nrot > MAXROT || (p.nrot & 1)) FN_FAIL("attn_kv4: nrot must be even and <= 128");
+    if (!(p.theta >= 1.0f)) FN_FAIL("attn_kv4: theta must be >= 1");
     if (p.nsplit < 1 || p.nsplit > 65535) FN_FAIL("attn_kv4: nsplit must be in 1..65535");
     if (p.max_blocks < 1 || p.max_blocks > 1 << 24) FN_FAIL("attn_kv4: max_blocks must be in 1..16777216");
     if (p.npages < 1 || p.npages > INT_MAX / PG) FN_FAIL("attn_kv4: npages must be in 1..33554431 (slots are 32-bit)");
@@ -533,10 +738,10 @@ int kv4_attn_launch(const Kv4Attn &p, hipStream_t st) {
     if (((uintptr_t) p.qg | (uintptr_t) p.k | (uintptr_t) p.v | (uintptr_t) p.wq | (uintptr_t) p.wk | (uintptr_t) p.cache |
          (uintptr_t) p.work | (uintptr_t) p.og) & 15)
         FN_FAIL("attn_kv4: qg, k, v, wq, wk, cache, work and og must be 16-byte aligned");
-    const int grp = p.nq / p.nkv, nrb = row_blocks(p.B, p.T, grp);
+    const int grp = p.nq / p.nkv, rt = item_rows(p.B, p.T, grp);
     if ((long long) p.T * grp > INT_MAX - 64) FN_FAIL("attn_kv4: too many query rows");
-    const size_t items = item_count(p.B, p.T, grp, 16 * nrb);
-    if (p.nkv > 65535 || items > 65535) FN_FAIL("attn_kv4: batch too large (at most 65535 items of 32 query rows)");
+    const size_t items = item_count(p.B, p.T, grp, rt);
+    if (p.nkv > 65535 || items > 65535) FN_FAIL("attn_kv4: batch too large (at most 65535 requests and pieces of 32 query rows)");
     if (p.work_bytes < kv4_work_bytes(p.B, p.T, p.nq, p.nkv, p.hd, p.nsplit)) FN_FAIL("attn_kv4: workspace too small");
     Kv4Args a{};
     a.B = p.B; a.T = p.T; a.nq = p.nq; a.nkv = p.nkv; a.grp = grp; a.mb = p.max_blocks; a.npages = p.npages;
@@ -544,21 +749,13 @@ int kv4_attn_launch(const Kv4Attn &p, hipStream_t st) {
     a.table = p.table; a.slot = p.slot; a.seq = p.seq; a.qg = p.qg; a.k = p.k; a.v = p.v; a.wq = p.wq; a.wk = p.wk;
     a.cache = p.cache; a.og = p.og;
     if (status_word(&a.status)) return -1;
-    const size_t rows = items * p.nkv * 16 * nrb;
     a.Q = static_cast<uint8_t *>(p.work);
-    a.part_o = reinterpret_cast<float *>(a.Q + rows * 1024);
-    a.part_ml = a.part_o + rows * p.nsplit * HD;
+    a.part_o = reinterpret_cast<float *>(a.Q + items * p.nkv * query_bytes(rt));
+    a.part_ml = a.part_o + items * p.nkv * rt * p.nsplit * HD;
     for (int i = 0; i < p.nrot / 2; ++i) a.freq[i] = std::pow((double) p.theta, -(2.0 * i) / p.nrot);
-    const dim3 grid(p.nsplit, p.nkv, (unsigned) items);
-    if (nrb == 1) {
-        hipLaunchKernelGGL(k_kv4_prep<16>, dim3(p.T), dim3(256), 0, st, a);
-        hipLaunchKernelGGL(k_attn_kv4<1>, grid, dim3(WAVES * 64), 0, st, a);
-        if (p.nsplit > 1) hipLaunchKernelGGL(k_kv4_combine<16>, dim3((unsigned) items * 4, p.nkv), dim3(256), 0, st, a);
-    } else {
-        hipLaunchKernelGGL(k_kv4_prep<32>, dim3(p.T), dim3(256), 0, st, a);
-        hipLaunchKernelGGL(k_attn_kv4<2>, grid, dim3(WAVES * 64), 0, st, a);
-        if (p.nsplit > 1) hipLaunchKernelGGL(k_kv4_combine<32>, dim3((unsigned) items * 8, p.nkv), dim3(256), 0, st, a);
-    }
+    if (rt == 8) launch<8>(a, st);
+    else if (rt == 16) launch<16>(a, st);
+    else launch<32>(a, st);
     FN_CK(hipGetLastError());
     return 0;
 }
