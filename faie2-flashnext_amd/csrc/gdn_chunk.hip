@@ -3,21 +3,23 @@
 // A token does S <- g S, d = beta (v - S^T k), S <- S + k d^T, o = S^T q / sqrt(dk).  Within a chunk of 64 tokens, with
 // G_i the sum of the log decays up to token i and S the state before the chunk, the updates d (rows of U) solve a
 // unit lower triangular system:
-//   U = M X,  X_i = beta_i (v_i - e^G_i S^T k_i),  M = (I + A)^-1,  A_ij = beta_i e^(G_i - G_j) k_i.k_j  (j < i)
+//   U = U0 - W S,  U0 = M diag(beta) V,  W = M diag(beta e^G) K,  M = (I + A)^-1,  A_ij = beta_i e^(G_i - G_j) k_i.k_j  (j < i)
 //   o_i = (e^G_i S^T q_i + sum_(j <= i) e^(G_i - G_j) q_i.k_j u_j) / sqrt(dk)
 //   S' = e^G_63 S + sum_j e^(G_63 - G_j) k_j u_j^T
-// so that only S -> S' is sequential, in steps of 64 tokens.  Two launches:
-//   k_chunk_intra, one workgroup a (chunk, key head), everything that does not need S: M and P_ij = e^(G_i - G_j) q_i.k_j of
+// so that only S -> S' is sequential, in steps of 64 tokens.  Two kinds of workgroups:
+//   k_chunk_intra, one a (chunk, key head), everything that does not need S: W, U0 and P_ij = e^(G_i - G_j) q_i.k_j of
 //     each value head that reads the key head, and q, k as matrix operands;
-//   k_chunk_scan, one workgroup a (request, value head, 32 columns of S), which walks the request's chunks with its
-//     columns of S in registers: five small products a chunk.
+//   k_chunk_scan, one a (request, value head, columns of S), which walks the request's chunks with its columns of S in
+//     registers: three small products one after the other a chunk, and two exchanges through the LDS.
+// W and U0 are formed before the scan, not M inside it: the scan is the sequential part, and M there is one more product
+// and exchange a chunk (15k tokens, 32 value heads: scan 596 us with M, 405 us with W; the other kernel 252 and 332 us).
 // Products: an fp32 operand is two f16 values (hi and lo, 11 bits each) under a power-of-two scale, and a product is hi
 // hi + hi lo + lo hi on v_mfma_f32_16x16x32_f16: what is left out is 2^-22 of a product at the worst and 2^-24 in the
 // mean, in half the instructions of six bf16 products and a fifth of the time of fp32 ones.  f16's range is met by
-// scales: one a row of q, k, M and P (they are factors of output rows, folded into the gates' factors), one a column
-// and 32 rows for S (from its largest value there), and bounds for X and U: |X| <= max beta max|v| + max(beta e^G |k|)
-// sqrt(128) max|S| in its column, |U| <= (largest row sum of |M|) of that.  A bound too large by a factor of up to 2^15
-// costs no bit of a value as large as the column's largest: f16 reaches 2^-24 and lo goes down to there.
+// scales: one a row of q, k, M, W and P (they are factors of output rows, folded into the gates' factors), one a column
+// of V, one a column and 32 rows of S (from its largest value there), and a bound for U: |U| <= max|U0| + max|W_i|
+// sqrt(128) max|S| in its column.  A bound too large by a factor of up to 2^15 costs no bit of a value as large as the
+// column's largest: f16 reaches 2^-24 and lo goes down to there.
 // Decays: G is summed in 64 bits, because differences of far sums are taken; all exponents are then <= 0 for decays < 1.
 #include "serve.cuh"
 
@@ -30,22 +32,23 @@ constexpr int C = 64;                         // tokens a chunk
 constexpr int RS = D + 4;                     // floats a row of q, k in the LDS
 constexpr int AS = C + 4, MS = 20;            // floats a row of A, of the diagonal blocks of M
 constexpr int FRAG = 1024;                    // an operand of one 16 x 16 x 32 product: 16 bytes a lane
-constexpr int KF = 0, QF = 32 * FRAG, KT = 64 * FRAG, KEY_BYTES = 96 * FRAG;    // a (chunk, key head)
-constexpr int MF = 0, PF = 16 * FRAG, GATES = 32 * FRAG, HEAD_BYTES = 34 * FRAG;  // a (chunk, value head)
-// GATES: [6][64] floats beta, beta e^G 2^ek, e^G 2^eq / sqrt(dk), e^(G63 - G) 2^ek, 2^ep / sqrt(dk), 2^em; then scalars
-constexpr int G_BETA = 0, G_KS = 64, G_QS = 128, G_UP = 192, G_P = 256, G_M = 320, G_SC = 384;
+constexpr int QF = 0, KT = 32 * FRAG, KEY_BYTES = 64 * FRAG;                         // a (chunk, key head)
+constexpr int WF = 0, U0 = 32 * FRAG, PF = 64 * FRAG, GATES = 80 * FRAG, HEAD_BYTES = 82 * FRAG;  // a (chunk, value head)
+// GATES: floats: [64] scale of W's row, e^G 2^eq / sqrt(dk), e^(G63 - G) 2^ek, 2^ep / sqrt(dk); [128] largest |U0| of a
+// column; sqrt(128) max|W_i|, largest e^(G63 - G) 2^ek, e^G63
+constexpr int G_W = 0, G_QS = 64, G_UP = 128, G_P = 192, G_UM = 256, G_SC = 384;
 constexpr float RSQRT_D = 0.08838834764831845f;
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 struct ChunkArgs {
     GdnChunk p;
     uint8_t *keys, *heads;  // the two parts of the workspace
-    int items;
 };
 
 __device__ __forceinline__ v4f mma(const v4u &a, const v4u &b, v4f c) {
@@ -56,8 +59,8 @@ __device__ __forceinline__ v4f mma(const v4u &a, const v4u &b, v4f c) {
 // wrong by a unit of hi: one element in some thousands, by 2^-11.)
 __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
     asm("" : "+v"(a), "+v"(b));
-    const h2 h = {(_Float16) a, (_Float16) b};
-    const h2 l = {(_Float16) (a - (float) h.x), (_Float16) (b - (float) h.y)};
+    const h2 h = __builtin_convertvector((v2f{a, b}), h2);
+    const h2 l = __builtin_convertvector((v2f{fmaf((float) h.x, -1.0f, a), fmaf((float) h.y, -1.0f, b)}), h2);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, l);
 }
@@ -78,10 +81,15 @@ __device__ __forceinline__ float silu_(float x) { return x * __builtin_amdgcn_rc
 
 __device__ __forceinline__ float4 lds4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 
+// grid (chunks, nkh), four waves.  What bounds it: memory.  15k tokens, 16 key and 32 value heads: 0.49 GB of q, k, v in,
+// 0.86 GB of operands out in 332 us, 4.1 TB/s.  M = (I + A)^-1 by blocks of 16: a wave inverts its diagonal block by
+// substitution, one column a lane, and forms its block row from the diagonal leftwards on fp32 matrix instructions.
 template <bool BLOCK>
 __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
-    __shared__ __align__(16) float rows[2][C * RS];            // q, k; later K operands | A, diagonal blocks of M
-    __shared__ float mul[2][C], back[2][C], kn[C], bet[C];     // row factors to f16's range and back, |k|, beta
+    __shared__ __align__(16) float rows[2][C * RS];            // q, k; later operands | A, diagonal blocks of M
+    __shared__ __align__(16) float mul[2][C], back[2][C];      // row factors to f16's range and back
+    __shared__ __align__(16) float bet[C], bks[C], mback[2][C];  // beta, beta e^G 2^ek; back of M's two forms
+    __shared__ float wam[4][C], wsq[4][C];                     // largest value and squares of W's rows, by wave
     __shared__ double G[C];
     const GdnChunk &p = a.p;
     const int item = blockIdx.x, kh = blockIdx.y;
@@ -145,12 +153,11 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
         if ((tid & 1) == 0) {
             mul[part][t] = nr * pow2(-e);
             back[part][t] = pow2(e);
-            if (part) kn[t] = sqrtf(ss) * nr;
         }
     }
     __syncthreads();
     // 2. operands.  Row operand (q, k): lane = row 16 wave + l%16, slot j of step s = dim 32 s + 16 (j / 4) + 4 (l / 16) + j % 4
-    v4u qh[4], ql[4], kh_[4], kl[4];
+    v4u qh[4], ql[4], kh_[4], kl[4], kt[2][2][2];
     {
         const int t = 16 * wave + r;
 #pragma unroll
@@ -160,13 +167,14 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
             for (int s = 0; s < 4; ++s) {
                 const float4 x = lds4(&rows[part][t * RS + 32 * s + 4 * q4]), y = lds4(&rows[part][t * RS + 32 * s + 16 + 4 * q4]);
                 const float v[8] = {x.x * m, x.y * m, x.z * m, x.w * m, y.x * m, y.y * m, y.z * m, y.w * m};
-                v4u hi, lo;
-                split8(v, hi, lo);
-                uint8_t *d = kd + (part ? KF : QF) + ((wave * 4 + s) * 2) * FRAG + lane * 16;
-                *reinterpret_cast<v4u *>(d) = hi;
-                *reinterpret_cast<v4u *>(d + FRAG) = lo;
-                if (part) kh_[s] = hi, kl[s] = lo;
-                else qh[s] = hi, ql[s] = lo;
+                if (part) {
+                    split8(v, kh_[s], kl[s]);
+                } else {
+                    split8(v, qh[s], ql[s]);
+                    uint8_t *d = kd + QF + ((wave * 4 + s) * 2) * FRAG + lane * 16;
+                    *reinterpret_cast<v4u *>(d) = qh[s];
+                    *reinterpret_cast<v4u *>(d + FRAG) = ql[s];
+                }
             }
         }
         // Column operand (k^T): lane = dim 32 wave + 16 c + l%16, slot j of step s = token 32 s + 16 (j / 4) + 4 (l / 16) + j % 4
@@ -180,19 +188,18 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                     const int u = 32 * s + 16 * (j / 4) + 4 * q4 + j % 4;
                     v[j] = rows[1][u * RS + 32 * wave + 16 * c + r] * mul[1][u];
                 }
-                v4u hi, lo;
-                split8(v, hi, lo);
+                split8(v, kt[c][s][0], kt[c][s][1]);
                 uint8_t *d = kd + KT + (((wave * 2 + c) * 2 + s) * 2) * FRAG + lane * 16;
-                *reinterpret_cast<v4u *>(d) = hi;
-                *reinterpret_cast<v4u *>(d + FRAG) = lo;
+                *reinterpret_cast<v4u *>(d) = kt[c][s][0];
+                *reinterpret_cast<v4u *>(d + FRAG) = kt[c][s][1];
             }
     }
     __syncthreads();
-    v4u *kop = reinterpret_cast<v4u *>(rows[0]);  // [tile][step][hi, lo][lane]
+    v4u *op = reinterpret_cast<v4u *>(rows[0]);  // [tile][step][hi, lo][lane]: K's row operands, later two forms of M
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        kop[((wave * 4 + s) * 2) * 64 + lane] = kh_[s];
-        kop[((wave * 4 + s) * 2 + 1) * 64 + lane] = kl[s];
+        op[((wave * 4 + s) * 2) * 64 + lane] = kh_[s];
+        op[((wave * 4 + s) * 2 + 1) * 64 + lane] = kl[s];
     }
     __syncthreads();
     // 3. k_j.k_i and k_j.q_i of the wave's 16 rows i (lane: i = 16 wave + l%16, j = 16 tile + 4 (l / 16) + e)
@@ -203,7 +210,7 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
         if (j <= wave) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const v4u h = kop[((j * 4 + s) * 2) * 64 + lane], l = kop[((j * 4 + s) * 2 + 1) * 64 + lane];
+                const v4u h = op[((j * 4 + s) * 2) * 64 + lane], l = op[((j * 4 + s) * 2 + 1) * 64 + lane];
                 kk[j] = mma(h, kl[s], kk[j]);
                 qk[j] = mma(h, ql[s], qk[j]);
                 kk[j] = mma(l, kh_[s], kk[j]);
@@ -223,9 +230,11 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
     }
     // 4. each value head of the key head
     float *A = rows[1], *Md = rows[1] + C * AS;
-    const int per = p.nvh / p.nkh;
+    const int per = p.nvh / p.nkh, Cc = 2 * p.nkh * D + p.nvh * D;
     for (int hi_ = 0; hi_ < per; ++hi_) {
         const int h = p.head_map == 0 ? kh + hi_ * p.nkh : kh * per + hi_;
+        uint8_t *hd = a.heads + ((size_t) item * p.nvh + h) * HEAD_BYTES;
+        float *gd = reinterpret_cast<float *>(hd + GATES);
         float be = 0.0f, g = 0.0f;
         if (lane < n) {
             const size_t t = row0 + lane;
@@ -245,47 +254,39 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
             const double y = __shfl_up(gs, d);
             if (lane >= d) gs += y;
         }
-        __syncthreads();  // the last head's A, Md, G and beta have been read (and K's operands)
-        if (wave == 0) {
-            G[lane] = gs;
-            bet[lane] = be;
-        }
-        uint8_t *hd = a.heads + ((size_t) item * p.nvh + h) * HEAD_BYTES;
-        float *gd = reinterpret_cast<float *>(hd + GATES);
+        __syncthreads();  // what the last head left in the LDS has been read
         if (wave == 0) {
             const double g63 = __shfl(gs, 63);
-            const float eg = expf((float) gs), up = expf((float) (g63 - gs)) * back[1][lane];
-            gd[G_BETA + lane] = be;
-            gd[G_KS + lane] = be * eg * back[1][lane];
+            const float eg = expf((float) gs), up = expf((float) (g63 - gs)) * back[1][lane], um = wave_max(up);
+            G[lane] = gs;
+            bet[lane] = be;
+            bks[lane] = be * eg * back[1][lane];
             gd[G_QS + lane] = eg * back[0][lane] * RSQRT_D;
             gd[G_UP + lane] = up;
-            const float bb = wave_max(fabsf(be)), bk = wave_max(fabsf(be) * eg * kn[lane]), um = wave_max(up);
             if (lane == 0) {
-                gd[G_SC] = bb;
-                gd[G_SC + 1] = bk * 11.3138f;  // sqrt(128), rounded up
-                gd[G_SC + 2] = um;
-                gd[G_SC + 3] = expf((float) g63);
+                gd[G_SC + 1] = um;
+                gd[G_SC + 2] = expf((float) g63);
             }
         }
         __syncthreads();
         const double gi = G[16 * wave + r];
         const float bi = bet[16 * wave + r];
-        float pv[4][4], pm = 0.0f;
+        {
+            float pv[4][4], pm = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float av[4];
+            for (int j = 0; j < 4; ++j) {
+                float av[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int jt = 16 * j + 4 * q4 + e, it = 16 * wave + r;
-                const float dec = j <= wave && jt <= it ? expf((float) (gi - G[jt])) : 0.0f;
-                av[e] = j <= wave && jt < it ? bi * dec * kk[j][e] : 0.0f;
-                pv[j][e] = j <= wave && jt <= it ? dec * qk[j][e] : 0.0f;
-                pm = fmaxf(pm, fabsf(pv[j][e]));
+                for (int e = 0; e < 4; ++e) {
+                    const int jt = 16 * j + 4 * q4 + e, it = 16 * wave + r;
+                    const float dec = j <= wave && jt <= it ? expf((float) (gi - G[jt])) : 0.0f;
+                    av[e] = j <= wave && jt < it ? bi * dec * kk[j][e] : 0.0f;
+                    pv[j][e] = j <= wave && jt <= it ? dec * qk[j][e] : 0.0f;
+                    pm = fmaxf(pm, fabsf(pv[j][e]));
+                }
+                if (j <= wave)
+                    *reinterpret_cast<float4 *>(A + (16 * wave + r) * AS + 16 * j + 4 * q4) = make_float4(av[0], av[1], av[2], av[3]);
             }
-            if (j <= wave)
-                *reinterpret_cast<float4 *>(A + (16 * wave + r) * AS + 16 * j + 4 * q4) = make_float4(av[0], av[1], av[2], av[3]);
-        }
-        {  // P's operand
             pm = max_quarters(pm);
             const int e = exp_of(pm) - 14;
             const float m = pow2(-e);
@@ -302,6 +303,50 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                     *reinterpret_cast<v4u *>(d) = hi;
                     *reinterpret_cast<v4u *>(d + FRAG) = lo;
                 }
+        }
+        // values of the wave's columns 32 wave + 16 c + l%16 (slots as in k^T), requested ahead
+        float vv[2][2][8];
+        if (BLOCK) {
+            const int ch0 = 2 * p.nkh * D + h * D + 32 * wave + r;
+            // rows behind the last, and before a request's first, read as 0; the latter are then taken from the ring
+            const brsrc xb = buf(p.qkv + (row0 - (t0 ? 3 : 0)) * Cc, (uint32_t) (n + (t0 ? 3 : 0)) * Cc * 4);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int ch = ch0 + 16 * c;
+                const float4 w = *reinterpret_cast<const float4 *>(p.conv_w + 4 * ch);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {  // four tokens in a row
+                    const int u0 = 16 * g + 4 * q4;
+                    float y[7];
+#pragma unroll
+                    for (int i = 0; i < 7; ++i) y[i] = bld(xb, (uint32_t) (((u0 + i - (t0 ? 0 : 3)) * Cc + ch) * 4), 0);
+                    if (g == 0 && t0 == 0 && q4 == 0) {
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)
+                            y[i] = p.conv_ring[((size_t) b * p.ring + ((p.pos[b] + i - 3) & (p.ring - 1))) * Cc + ch];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float z = w.x * y[i];
+                        z = fmaf(w.y, y[i + 1], z);
+                        z = fmaf(w.z, y[i + 2], z);
+                        z = fmaf(w.w, y[i + 3], z);
+                        vv[c][g / 2][4 * (g % 2) + i] = u0 + i < n ? silu_(z) : 0.0f;
+                    }
+                    if (g % 2) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        } else {
+            const brsrc v = buf(p.v + row0 * p.nvh * D + h * D, (uint32_t) ((n - 1) * p.nvh * D + D) * 4);  // rows behind: 0
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int u = 32 * s + 16 * (j / 4) + 4 * q4 + j % 4;
+                        vv[c][s][j] = bld(v, (uint32_t) (u * p.nvh * D + 32 * wave + 16 * c + r) * 4, 0);
+                    }
         }
         __syncthreads();
         {  // the inverse of the wave's diagonal block, lane = column l%16, by substitution
@@ -348,296 +393,404 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                 o = __builtin_amdgcn_mfma_f32_16x16x4f32(Md[(16 * j + 4 * q4 + e) * MS + r], t[e], o, 0, 0, 0);
             mt[j] = -o;
         }
-        {  // M's operand
-            float am = 0.0f, sum = 0.0f;
+        // M diag(beta e^G 2^ek) and M diag(beta) as operands, a scale a row
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int f = 0; f < 2; ++f) {
+            float am = 0.0f, v[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 x = lds4((f ? bet : bks) + 16 * j + 4 * q4);
+                const float y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    am = fmaxf(am, fabsf(mt[j][e]));
-                    sum += fabsf(mt[j][e]);
+                    v[j][e] = mt[j][e] * y[e];
+                    am = fmaxf(am, fabsf(v[j][e]));
                 }
+            }
             am = max_quarters(am);
-            sum = row_max(sum_quarters(sum));
             const int e = exp_of(am) - 14;
             const float m = pow2(-e);
-            if (q4 == 0) gd[G_M + 16 * wave + r] = pow2(e);
-            if (lane == 0) gd[G_SC + 4 + wave] = sum;
+            if (q4 == 0) mback[f][16 * wave + r] = pow2(e);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
                 if (2 * s <= wave) {
-                    float v[8];
+                    float x[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = mt[2 * s + j / 4][j % 4] * m;
-                    v4u hi, lo;
-                    split8(v, hi, lo);
-                    uint8_t *d = hd + MF + ((wave * 2 + s) * 2) * FRAG + lane * 16;
-                    *reinterpret_cast<v4u *>(d) = hi;
-                    *reinterpret_cast<v4u *>(d + FRAG) = lo;
+                    for (int j = 0; j < 8; ++j) x[j] = v[2 * s + j / 4][j % 4] * m;
+                    v4u *d = op + (((f * 4 + wave) * 2 + s) * 2) * 64 + lane;
+                    split8(x, d[0], d[64]);
                 }
+        }
+        __syncthreads();
+        const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        // U0 of the wave's columns: lane = column, tokens 16 i + 4 (l / 16) + e
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float am = 0.0f, um = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) am = fmaxf(am, fabsf(vv[c][s][j]));
+            am = max_quarters(am);
+            const int e = exp_of(am) - 14;
+            const float m = pow2(-e), f = pow2(e);
+            v4u vh[2], vl[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) vv[c][s][j] *= m;
+                split8(vv[c][s], vh[s], vl[s]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v4f u = zero;
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+                    if (2 * s <= i) {
+                        const v4u mh = op[(((4 + i) * 2 + s) * 2) * 64 + lane], ml = op[(((4 + i) * 2 + s) * 2 + 1) * 64 + lane];
+                        u = mma(mh, vl[s], u);
+                        u = mma(ml, vh[s], u);
+                        u = mma(mh, vh[s], u);
+                    }
+                const float4 bk = lds4(&mback[1][16 * i + 4 * q4]);
+                const float4 o = make_float4(u[0] * bk.x * f, u[1] * bk.y * f, u[2] * bk.z * f, u[3] * bk.w * f);
+                um = fmaxf(um, fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w))));
+                *reinterpret_cast<float4 *>(hd + U0 + ((i * 8 + 2 * wave + c) * 64 + lane) * 16) = o;
+            }
+            um = max_quarters(um);
+            if (q4 == 0) gd[G_UM + 32 * wave + 16 * c + r] = um;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // W^T = K^T (M diag)^T of the wave's dims, all tokens: lane = token 16 i + l%16, dims 32 wave + 16 c + 4 (l / 16) + e
+        v4f w[2][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[0][i] = w[1][i] = zero;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                if (2 * s <= i) {
+                    const v4u mh = op[((i * 2 + s) * 2) * 64 + lane], ml = op[((i * 2 + s) * 2 + 1) * 64 + lane];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        w[c][i] = mma(kt[c][s][0], ml, w[c][i]);
+                        w[c][i] = mma(kt[c][s][1], mh, w[c][i]);
+                        w[c][i] = mma(kt[c][s][0], mh, w[c][i]);
+                    }
+                }
+            const float f = mback[0][16 * i + r];
+            w[0][i] *= f;
+            w[1][i] *= f;
+            float am = 0.0f, sq = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    am = fmaxf(am, fabsf(w[c][i][e]));
+                    sq = fmaf(w[c][i][e], w[c][i][e], sq);
+                }
+            am = max_quarters(am);
+            sq = sum_quarters(sq);
+            if (q4 == 0) {
+                wam[wave][16 * i + r] = am;
+                wsq[wave][16 * i + r] = sq;
+            }
+        }
+        __syncthreads();
+        // W as the scan's row operand: step `wave` of every row tile
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 16 * i + r;
+            const float am = fmaxf(fmaxf(wam[0][t], wam[1][t]), fmaxf(wam[2][t], wam[3][t]));
+            const int e = exp_of(am) - 14;
+            const float m = pow2(-e);
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = w[j / 4][i][j % 4] * m;
+            v4u hi, lo;
+            split8(x, hi, lo);
+            uint8_t *d = hd + WF + ((i * 4 + wave) * 2) * FRAG + lane * 16;
+            *reinterpret_cast<v4u *>(d) = hi;
+            *reinterpret_cast<v4u *>(d + FRAG) = lo;
+            if (wave == 0 && q4 == 0) gd[G_W + t] = pow2(e);
+        }
+        if (wave == 1) {
+            const float n2 = wave_max((wsq[0][lane] + wsq[1][lane]) + (wsq[2][lane] + wsq[3][lane]));
+            if (lane == 0) gd[G_SC] = sqrtf(n2) * 11.3138f;  // sqrt(128), rounded up
         }
     }
 }
 
-// grid (nvh, D / (16 NC), B), four waves.  Wave w owns tokens 16 w .. + 15 of X, U and o, and rows 32 w .. + 31 of S; lane = column
-// l%16 of each of NC column tiles, rows 4 (l / 16) + e.  That is also the layout of an operand's slots, so what a wave
-// computes it splits and writes to the LDS as it stands, and the others read whole operands: S, X and U meet there once
-// a chunk each, with one barrier.
-template <bool BLOCK, int NC>
-__global__ void __launch_bounds__(256, 1) k_chunk_scan(const ChunkArgs a) {
+// grid (nvh, D / (16 NC), B), nine waves.  Waves 0..3 carry the state: wave w owns tokens 16 w .. + 15 of U and rows 32 w
+// .. + 31 of S.  Waves 4..7 compute the outputs of tokens 16 (w - 4) .. + 15.  Lane = column l%16 of each of NC column
+// tiles, rows 4 (l / 16) + e.  That is also the layout of an operand's slots, so what a wave computes it splits and writes
+// to the LDS as it stands, and the others read whole operands: S and U meet there once a chunk each, with one barrier.
+//   state waves:   | U = U0 - W S, written | S' = e^G63 S + K^T U, written |
+//   output waves:  | S^T q                 | + P U, stored                 |
+// Operands are requested a chunk ahead, each as soon as its registers are free, and between other work, because a wave
+// stops at a load that the address unit cannot take yet.  That reaches over the L2's latency, not the memory's, and the
+// workgroups of a head read the same operands at the same time.  So wave 8 touches the operands two chunks ahead, each of
+// the head's workgroups (which share an XCD where nvh is a multiple of 8) its part of the lines: 538 us without it, 405 us
+// with it at 15k tokens and 32 heads.
+// What bounds it then: the way round the state waves, 1.3 us a chunk of 1.7: two barriers, two trips through the LDS and
+// the products between them; the rest is the operands' 113 KiB a chunk, whatever the columns, at 64 bytes a cycle and CU.
+// That is why two column tiles (2.7 us a chunk) are taken as soon as one would leave more workgroups than CUs.
+template <int NC>
+__global__ void __launch_bounds__(576, 3) k_chunk_scan(const ChunkArgs a) {
     __shared__ v4u Sop[4][NC][2][64];                   // [32 rows][column tile][hi, lo][lane]
-    __shared__ v4u Xop[2][NC][2][64], Uop[2][NC][2][64], Wop[2][NC][2][64];  // [32 tokens]...: X, U, e^(G63 - G) U
-    __shared__ float smax[4][NC][16], sinv[4][NC][16], vmax[4][NC][16];
+    __shared__ v4u Uop[2][NC][2][64], Wop[2][NC][2][64];  // [32 tokens]...: U, e^(G63 - G) U
+    __shared__ float smax[4][NC][16], sinv[4][NC][16];
+    constexpr int NG = (G_SC + 4) / 4;                  // the chunk's factors pass through the LDS, a chunk ahead
+    __shared__ __align__(16) float gates[2][NG * 4];
     const GdnChunk &p = a.p;
     const int h = blockIdx.x, col0 = blockIdx.y * 16 * NC, b = blockIdx.z;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
+    const int role = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int lane = threadIdx.x & 63, r = lane & 15, q4 = lane >> 4;
     const int c0 = p.cu[b], len = min(p.cu[b + 1], p.T) - c0;
     if (c0 < 0 || len <= 0) return;
     const int per = p.nvh / p.nkh, kh = p.head_map == 0 ? h % p.nkh : h / per;
     const int item0 = first_item(p.cu, b, 1, C), chunks = (len + C - 1) / C;
-    const int Cc = 2 * p.nkh * D + p.nvh * D;
-    float s[NC][2][4];
-    float *Sg = p.S + ((size_t) b * p.nvh + h) * D * D + col0 + r;
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][c][e] = Sg[(32 * wave + 16 * c + 4 * q4 + e) * D + 16 * n];
-    float4 cw[NC];
-    if (BLOCK) {
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-            cw[n] = *reinterpret_cast<const float4 *>(p.conv_w + 4 * (2 * p.nkh * D + h * D + col0 + 16 * n + r));
-    }
-    v4u kf[4][2], qf[4][2], mf[2][2], pf[2][2], kt[2][2][2];
-    float v[NC][7];
-    auto key = [&](int i) { return a.keys + ((size_t) (item0 + i) * p.nkh + kh) * KEY_BYTES + lane * 16; };
-    auto head = [&](int i) { return a.heads + ((size_t) (item0 + i) * p.nvh + h) * HEAD_BYTES; };
-    auto ld = [&](const uint8_t *x) { return *reinterpret_cast<const v4u *>(x); };
-    auto load_rows = [&](int i, int at, v4u(&f)[4][2]) {
-        const uint8_t *x = key(i) + at + wave * 8 * FRAG;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j / 2][j % 2] = ld(x + j * FRAG);
-    };
-    auto load_tri = [&](int i, int at, v4u(&f)[2][2]) {
-        const uint8_t *x = head(i) + at + wave * 4 * FRAG + lane * 16;
-        f[0][0] = ld(x);
-        f[0][1] = ld(x + FRAG);
-        if (wave >= 2) {
-            f[1][0] = ld(x + 2 * FRAG);
-            f[1][1] = ld(x + 3 * FRAG);
-        }
-    };
-    auto load_kt = [&](int i) {
-        const uint8_t *x = key(i) + KT + wave * 8 * FRAG;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) kt[j / 4][j / 2 % 2][j % 2] = ld(x + j * FRAG);
-    };
-    // the chunk's values of the lane's tokens 16 wave + 4 q4 + e; BLOCK: raw inputs from three tokens before
-    auto load_v = [&](int i) {
-        const int t = i * C + 16 * wave + 4 * q4;
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-#pragma unroll
-            for (int e = 0; e < (BLOCK ? 7 : 4); ++e) {
-                const int u = BLOCK ? t + e - 3 : t + e;
-                const int col = (BLOCK ? 2 * p.nkh * D : 0) + h * D + col0 + 16 * n + r;
-                v[n][e] = 0.0f;
-                if (u < len) {
-                    if (!BLOCK) v[n][e] = p.v[(size_t) (c0 + u) * p.nvh * D + col];
-                    else if (u >= 0) v[n][e] = p.qkv[(size_t) (c0 + u) * Cc + col];
-                    else v[n][e] = p.conv_ring[((size_t) b * p.ring + ((p.pos[b] + u) & (p.ring - 1))) * Cc + col];
-                }
-            }
-    };
-    float val[NC][4];
-    auto take_v = [&](int i) {  // values, and their largest in the column
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            float am = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (BLOCK) {
-                    float y = cw[n].x * v[n][e];
-                    y = fmaf(cw[n].y, v[n][e + 1], y);
-                    y = fmaf(cw[n].z, v[n][e + 2], y);
-                    y = fmaf(cw[n].w, v[n][e + 3], y);
-                    val[n][e] = i * C + 16 * wave + 4 * q4 + e < len ? silu_(y) : 0.0f;
-                } else {
-                    val[n][e] = v[n][e];
-                }
-                am = fmaxf(am, fabsf(val[n][e]));
-            }
-            am = max_quarters(am);
-            if (q4 == 0) vmax[wave][n][r] = am;
-        }
-    };
-    auto put_s = [&]() {
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            float am = 0.0f, x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) am = fmaxf(am, fabsf(s[n][j / 4][j % 4]));
-            am = max_quarters(am);
-            const int e = exp_of(am) - 14;
-            const float m = pow2(-e);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = s[n][j / 4][j % 4] * m;
-            split8(x, Sop[wave][n][0][lane], Sop[wave][n][1][lane]);
-            if (q4 == 0) {
-                smax[wave][n][r] = am;
-                sinv[wave][n][r] = pow2(e);
-            }
-        }
-    };
-    auto put4 = [&](v4u(&op)[2][NC][2][64], int n, const float (&x)[4], float m) {  // the wave's 16 tokens of an operand
-        uint32_t hi[2], lo[2];
-        split2(x[0] * m, x[1] * m, hi[0], lo[0]);
-        split2(x[2] * m, x[3] * m, hi[1], lo[1]);
-        reinterpret_cast<v2u *>(&op[wave / 2][n][0][lane])[wave & 1] = v2u{hi[0], hi[1]};
-        reinterpret_cast<v2u *>(&op[wave / 2][n][1][lane])[wave & 1] = v2u{lo[0], lo[1]};
-    };
-    load_v(0);
-    load_rows(0, KF, kf);
-    load_rows(0, QF, qf);
-    load_tri(0, MF, mf);
-    load_kt(0);
-    load_tri(0, PF, pf);
-    take_v(0);
-    put_s();
+    const int tok = 16 * wave + 4 * q4;  // the lane's first token
+    const uint32_t lane16 = lane * 16;
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < chunks; ++i) {
-        const int nx = min(i + 1, chunks - 1);
-        const float *gd = reinterpret_cast<const float *>(head(i) + GATES);
-        const int tok = 16 * wave + 4 * q4;
-        const float4 beta4 = *reinterpret_cast<const float4 *>(gd + G_BETA + tok), ks4 = *reinterpret_cast<const float4 *>(gd + G_KS + tok);
-        const float4 qs4 = *reinterpret_cast<const float4 *>(gd + G_QS + tok), up4 = *reinterpret_cast<const float4 *>(gd + G_UP + tok);
-        const float4 p4 = *reinterpret_cast<const float4 *>(gd + G_P + tok), m4 = *reinterpret_cast<const float4 *>(gd + G_M + tok);
-        const float4 sc = *reinterpret_cast<const float4 *>(gd + G_SC), mn4 = *reinterpret_cast<const float4 *>(gd + G_SC + 4);
-        const float bt[4] = {beta4.x, beta4.y, beta4.z, beta4.w}, ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
-        const float qs[4] = {qs4.x, qs4.y, qs4.z, qs4.w}, up[4] = {up4.x, up4.y, up4.z, up4.w};
-        const float pp[4] = {p4.x, p4.y, p4.z, p4.w}, mm[4] = {m4.x, m4.y, m4.z, m4.w};
-        const float mnorm = fmaxf(fmaxf(mn4.x, mn4.y), fmaxf(mn4.z, mn4.w));
-        lds_barrier();  // S (and the largest values of the columns) is there
-        float si[4][NC], xb[NC];
+    auto key = [&](int i) __attribute__((always_inline)) {
+        return buf(a.keys + ((size_t) (item0 + i) * p.nkh + kh) * KEY_BYTES, KEY_BYTES);
+    };
+    auto head = [&](int i) __attribute__((always_inline)) {
+        return buf(a.heads + ((size_t) (item0 + i) * p.nvh + h) * HEAD_BYTES, HEAD_BYTES);
+    };
+    auto ld = [&](brsrc d, int at) __attribute__((always_inline)) {
+        return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(d, (int) lane16, at, 0));
+    };
+    auto load_rows = [&](brsrc d, int at, v4u(&f)[4][2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j / 2][j % 2] = ld(d, at + (wave * 8 + j) * FRAG);
+    };
+    // largest |U| of the columns (a bound) from the largest |S|, and the scales of S's 32-row steps
+    auto bounds = [&](const float *gd, float sc, float(&si)[4][NC], float(&ub)[NC]) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            float sm = 0.0f, vm = 0.0f;
+            float sm = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 sm = fmaxf(sm, smax[w][n][r]);
-                vm = fmaxf(vm, vmax[w][n][r]);
                 si[w][n] = sinv[w][n][r];
             }
-            xb[n] = fmaf(sc.x, vm, sc.y * sm);
+            ub[n] = fmaf(sc, sm, gd[G_UM + col0 + 16 * n + r]);
         }
-        v4f ka[NC], qa[NC];
-#pragma unroll
-        for (int n = 0; n < NC; ++n) ka[n] = qa[n] = zero;
-        v4u sh[4][NC], sl[4][NC];
+    };
+    // S^T f of the wave's rows: the 32-row steps have scales of their own, so each is summed apart (which also keeps
+    // products that wait for each other apart)
+    auto times_s = [&](const v4u(&f)[4][2], const float(&si)[4][NC], v4f(&acc)[NC]) __attribute__((always_inline)) {
+        v4f t[4][NC];
+        v4u sh[4][NC];
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 sh[w][n] = Sop[w][n][0][lane];
-                sl[w][n] = Sop[w][n][1][lane];
-                v4f t = mma(kf[w][0], sl[w][n], zero);
-                t = mma(kf[w][1], sh[w][n], t);
-                t = mma(kf[w][0], sh[w][n], t);
-                ka[n] += t * si[w][n];
+                t[w][n] = mma(f[w][1], sh[w][n], zero);
             }
-        load_rows(nx, KF, kf);
-        int ex[NC];
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            float x[4];
-            ex[n] = exp_of(xb[n]) - 14;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = bt[e] * val[n][e] - ks[e] * ka[n][e];
-            put4(Xop, n, x, pow2(-ex[n]));
-        }
-        load_v(nx);
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
+            for (int n = 0; n < NC; ++n) t[w][n] = mma(f[w][0], Sop[w][n][1][lane], t[w][n]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int n = 0; n < NC; ++n) t[w][n] = mma(f[w][0], sh[w][n], t[w][n]);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) acc[n] = (t[0][n] * si[0][n] + t[1][n] * si[1][n]) + (t[2][n] * si[2][n] + t[3][n] * si[3][n]);
+    };
+    if (role == 2) {
+        __shared__ uint32_t sink[64];  // loads to the LDS hold no registers; what they leave here is not read
+        auto touch = [&](int i) __attribute__((always_inline)) {
+            const brsrc hd = head(i), kd = key(i);
+            auto *to = (__attribute__((address_space(3))) void *) sink;
+            for (int l = blockIdx.y * 64 + lane; l < HEAD_BYTES / 128; l += D / 16 / NC * 64)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(hd, to, 4, l * 128, 0, 0, 0);
+            for (int l = blockIdx.y * 64 + lane; l < KEY_BYTES / 128; l += D / 16 / NC * 64)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(kd, to, 4, l * 128, 0, 0, 0);
+        };
+        touch(min(1, chunks - 1));
+        for (int i = 0; i < chunks; ++i) {
+            lds_barrier();
+            touch(min(i + 2, chunks - 1));
+            lds_barrier();
+        }
+        __builtin_amdgcn_s_waitcnt(0);  // the LDS is the workgroup's until they have come
+    } else if (role == 0) {
+        float s[NC][2][4];
+        float *Sg = p.S + ((size_t) b * p.nvh + h) * D * D + col0 + r;
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][c][e] = Sg[(32 * wave + 16 * c + 4 * q4 + e) * D + 16 * n];
+        v4u wf[4][2], kt[2][2][2];
+        float4 u0[NC];
+        auto load_kt = [&](brsrc d) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) kt[j / 4][j / 2 % 2][j % 2] = ld(d, KT + (wave * 8 + j) * FRAG);
+        };
+        auto load_u0 = [&](brsrc d) __attribute__((always_inline)) {
+#pragma unroll
+            for (int n = 0; n < NC; ++n) u0[n] = bld4(d, lane16, U0 + (wave * 8 + blockIdx.y * NC + n) * FRAG);
+        };
+        auto put_s = [&]() __attribute__((always_inline)) {
+#pragma unroll
             for (int n = 0; n < NC; ++n) {
-                v4f t = mma(qf[w][0], sl[w][n], zero);
-                t = mma(qf[w][1], sh[w][n], t);
-                t = mma(qf[w][0], sh[w][n], t);
-                qa[n] += t * si[w][n];
-            }
-        load_rows(nx, QF, qf);
-        lds_barrier();  // X is there
+                float am = 0.0f, x[8];
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            v4f u = zero;
+                for (int j = 0; j < 8; ++j) am = fmaxf(am, fabsf(s[n][j / 4][j % 4]));
+                am = max_quarters(am);
+                const int e = exp_of(am) - 14;
+                const float m = pow2(-e);
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
-                if (2 * w <= wave) {
-                    const v4u xh = Xop[w][n][0][lane], xl = Xop[w][n][1][lane];
-                    u = mma(mf[w][0], xl, u);
-                    u = mma(mf[w][1], xh, u);
-                    u = mma(mf[w][0], xh, u);
+                for (int j = 0; j < 8; ++j) x[j] = s[n][j / 4][j % 4] * m;
+                split8(x, Sop[wave][n][0][lane], Sop[wave][n][1][lane]);
+                if (q4 == 0) {
+                    smax[wave][n][r] = am;
+                    sinv[wave][n][r] = pow2(e);
                 }
-            const float f = pow2(ex[n]), ub = xb[n] * mnorm;
-            float x[4], y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = u[e] * (mm[e] * f);
-                y[e] = x[e] * up[e];
             }
-            put4(Uop, n, x, pow2(14 - exp_of(ub)));
-            put4(Wop, n, y, pow2(14 - exp_of(ub * sc.z)));
-        }
-        load_tri(nx, MF, mf);
-        lds_barrier();  // U is there
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const float f = pow2(exp_of(xb[n] * mnorm * sc.z) - 14);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                v4f t = zero;
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const v4u uh = Wop[w][n][0][lane], ul = Wop[w][n][1][lane];
-                    t = mma(kt[c][w][0], ul, t);
-                    t = mma(kt[c][w][1], uh, t);
-                    t = mma(kt[c][w][0], uh, t);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][c][e] = fmaf(t[e], f, sc.w * s[n][c][e]);
-            }
-        }
-        load_kt(nx);
-        take_v(nx);
+        };
+        auto put4 = [&](v4u(&op)[2][NC][2][64], int n, const float(&x)[4], float m) __attribute__((always_inline)) {
+            uint32_t hi[2], lo[2];  // the wave's 16 tokens of an operand
+            split2(x[0] * m, x[1] * m, hi[0], lo[0]);
+            split2(x[2] * m, x[3] * m, hi[1], lo[1]);
+            reinterpret_cast<v2u *>(&op[wave / 2][n][0][lane])[wave & 1] = v2u{hi[0], hi[1]};
+            reinterpret_cast<v2u *>(&op[wave / 2][n][1][lane])[wave & 1] = v2u{lo[0], lo[1]};
+        };
+        // in the order of the loop's requests: its waits count them as both ways into it have them
+        load_u0(head(0));
+        __builtin_amdgcn_sched_barrier(0);
+        load_rows(head(0), WF, wf);
+        __builtin_amdgcn_sched_barrier(0);
+        load_kt(key(0));
+        __builtin_amdgcn_sched_barrier(0);
         put_s();
+        for (int i = 0; i < chunks; ++i) {
+            const int nx = min(i + 1, chunks - 1);
+            const float *gd = gates[i & 1];
+            const brsrc hn = head(nx), kn = key(nx);
+            lds_barrier();  // S (and the largest values of the columns) is there
+            const float4 sc = lds4(gd + G_SC);
+            float si[4][NC], ub[NC];
+            bounds(gd, sc.x, si, ub);
+            v4f wa[NC];
+            times_s(wf, si, wa);
+            __builtin_amdgcn_sched_barrier(0);
+            float fs[NC];
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const float f = pow2(exp_of(xb[n] * mnorm) - 14);
-            v4f t = zero;
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-                if (2 * w <= wave) {
-                    const v4u uh = Uop[w][n][0][lane], ul = Uop[w][n][1][lane];
-                    t = mma(pf[w][0], ul, t);
-                    t = mma(pf[w][1], uh, t);
-                    t = mma(pf[w][0], uh, t);
-                }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int u = i * C + tok + e;
-                if (u < len) p.o[((size_t) (c0 + u) * p.nvh + h) * D + col0 + 16 * n + r] = fmaf(qs[e], qa[n][e], pp[e] * f * t[e]);
+            for (int n = 0; n < NC; ++n) {
+                const float4 fw = lds4(gd + G_W + tok), up = lds4(gd + G_UP + tok);
+                const float x[4] = {u0[n].x - fw.x * wa[n][0], u0[n].y - fw.y * wa[n][1], u0[n].z - fw.z * wa[n][2],
+                                    u0[n].w - fw.w * wa[n][3]};
+                const float y[4] = {x[0] * up.x, x[1] * up.y, x[2] * up.z, x[3] * up.w};
+                const int ew = exp_of(ub[n] * sc.y) - 14;
+                fs[n] = pow2(ew);
+                put4(Uop, n, x, pow2(14 - exp_of(ub[n])));
+                put4(Wop, n, y, pow2(-ew));
             }
+            load_u0(hn);
+            __builtin_amdgcn_sched_barrier(0);
+            lds_barrier();  // U is there
+            load_rows(hn, WF, wf);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                v4f t[2][2];  // [16 rows][32 tokens]
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) t[c][w] = mma(kt[c][w][q == 1], Wop[w][n][q == 0][lane], q == 0 ? zero : t[c][w]);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][c][e] = fmaf(t[c][0][e] + t[c][1][e], fs[n], sc.z * s[n][c][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_kt(kn);
+            put_s();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 8 * NC, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        load_tri(nx, PF, pf);
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) Sg[(32 * wave + 16 * c + 4 * q4 + e) * D + 16 * n] = s[n][c][e];
+    } else {
+        v4u qf[4][2], pf[2][2];
+        float4 gate;
+        const int gt = threadIdx.x & 255;
+        auto load_p = [&](brsrc d) __attribute__((always_inline)) {
+            pf[0][0] = ld(d, PF + wave * 4 * FRAG);
+            pf[0][1] = ld(d, PF + wave * 4 * FRAG + FRAG);
+            if (wave >= 2) {
+                pf[1][0] = ld(d, PF + wave * 4 * FRAG + 2 * FRAG);
+                pf[1][1] = ld(d, PF + wave * 4 * FRAG + 3 * FRAG);
+            }
+        };
+        auto load_gates = [&](brsrc d) __attribute__((always_inline)) {
+            if (gt < NG) gate = bld4(d, gt * 16, GATES);
+        };
+        auto put_gates = [&](int i) __attribute__((always_inline)) {
+            if (gt < NG) reinterpret_cast<float4 *>(gates[i & 1])[gt] = gate;
+        };
+        load_gates(head(0));
+        put_gates(0);
+        load_rows(key(0), QF, qf);
+        __builtin_amdgcn_sched_barrier(0);
+        load_p(head(0));
+        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < chunks; ++i) {
+            const int nx = min(i + 1, chunks - 1);
+            const float *gd = gates[i & 1];
+            const brsrc hn = head(nx), kn = key(nx);
+            load_gates(hn);
+            lds_barrier();  // S (and the largest values of the columns) is there
+            float si[4][NC], ub[NC];
+            bounds(gd, gd[G_SC], si, ub);
+            v4f qa[NC];
+            times_s(qf, si, qa);
+            __builtin_amdgcn_sched_barrier(0);
+            load_rows(kn, QF, qf);
+            put_gates(nx);
+            __builtin_amdgcn_sched_barrier(0);
+            lds_barrier();  // U is there
+            const brsrc od = buf(p.o + ((size_t) (c0 + i * C) * p.nvh + h) * D + col0,
+                                 (uint32_t) (min(len - i * C, C) - 1) * p.nvh * D * 4 + 16 * NC * 4);  // rows behind the last: dropped
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                // the wave's rows of P times U (tokens 32 .. only for the rows behind them)
+                const v4u uh = Uop[0][n][0][lane], ul = Uop[0][n][1][lane];
+                v4f t = mma(pf[0][0], ul, zero), t2 = mma(pf[0][1], uh, zero);
+                if (wave >= 2) {
+                    const v4u uh1 = Uop[1][n][0][lane], ul1 = Uop[1][n][1][lane];
+                    t = mma(pf[1][0], ul1, t);
+                    t2 = mma(pf[1][1], uh1, t2);
+                    t2 = mma(pf[1][0], uh1, t2);
+                }
+                t = mma(pf[0][0], uh, t);
+                t += t2;
+                const float4 qs4 = lds4(gd + G_QS + tok), pp4 = lds4(gd + G_P + tok);
+                const float qs[4] = {qs4.x, qs4.y, qs4.z, qs4.w}, pp[4] = {pp4.x, pp4.y, pp4.z, pp4.w};
+                const float f = pow2(exp_of(ub[n]) - 14);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    bst(od, (uint32_t) (tok + e) * p.nvh * D * 4 + 64 * n + 4 * r, 0, fmaf(qs[e], qa[n][e], pp[e] * f * t[e]));
+            }
+            load_p(hn);
+        }
     }
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) Sg[(32 * wave + 16 * c + 4 * q4 + e) * D + 16 * n] = s[n][c][e];
 }
 
 // The fused block's end: gated RMSNorm of every (token, value head) in place, 32 lanes a row; and, in the blocks behind
@@ -697,22 +850,26 @@ int gdn_chunk_launch(const GdnChunk &p, hipStream_t st) {
         FN_FAIL(block ? "gdn_chunk: conv_w, z, norm_w, out and work must be 16-byte aligned"
                       : "gdn_chunk: q, k, o and work must be 16-byte aligned");
     if (p.work_bytes < gdn_chunk_work_bytes(p.B, p.T, p.nkh, p.nvh)) FN_FAIL("gdn_chunk: workspace too small");
-    ChunkArgs a{p, nullptr, nullptr, 0};
+    ChunkArgs a{p, nullptr, nullptr};
     const size_t items = item_count(p.B, p.T, 1, C);
-    a.items = (int) items;
     a.keys = static_cast<uint8_t *>(p.work);
     a.heads = a.keys + items * p.nkh * KEY_BYTES;
-    const dim3 gi((unsigned) items, p.nkh), gs(p.nvh, D / 32, p.B);
+    // columns a scan workgroup (above): one tile while every workgroup has a CU of its own.  48 value heads of one request:
+    // 277 us with one tile, 174 us with two; 32 value heads: 405 us with one (256 workgroups, 1.7 us a chunk), 2.7 us a
+    // chunk with two
+    const int nc = (long long) p.B * p.nvh * (D / 16) > device_cus() ? 2 : 1;
+    const dim3 gi((unsigned) items, p.nkh), gs(p.nvh, D / 16 / nc, p.B);
+    auto *scan = nc == 1 ? k_chunk_scan<1> : k_chunk_scan<2>;
     const size_t norm = ((size_t) p.T * p.nvh + 7) / 8;                                   // blocks of k_chunk_finish
     const size_t ring = p.B * ((((size_t) 2 * p.nkh + p.nvh) * D + 255) / 256);
     if (norm + ring > 0x7fffffffu) FN_FAIL("gdn_chunk: too many rows");
     if (block) {
         hipLaunchKernelGGL(k_chunk_intra<true>, gi, dim3(256), 0, st, a);
-        hipLaunchKernelGGL((k_chunk_scan<true, 2>), gs, dim3(256), 0, st, a);
+        hipLaunchKernelGGL(scan, gs, dim3(576), 0, st, a);
         hipLaunchKernelGGL(k_chunk_finish, dim3((unsigned) (norm + ring)), dim3(256), 0, st, a, (unsigned) norm);
     } else {
         hipLaunchKernelGGL(k_chunk_intra<false>, gi, dim3(256), 0, st, a);
-        hipLaunchKernelGGL((k_chunk_scan<false, 2>), gs, dim3(256), 0, st, a);
+        hipLaunchKernelGGL(scan, gs, dim3(576), 0, st, a);
     }
     FN_CK(hipGetLastError());
     return 0;
