@@ -18,7 +18,8 @@ constexpr int FRAG = 64 * 24;                          // a part's operand: 16 b
 constexpr int QBLK = 2 * NPART * FRAG + 2 * 64 * 8;    // 16 query rows: [half][part] operands, [half] scales
 constexpr int HSLOT = 3;                               // 8 query rows: columns 0..7 hold parts 0..2, 8..15 parts 3, 4, zero
 constexpr int HBLK = 2 * HSLOT * FRAG + 2 * 64 * 4;    // [half][slot] operands, [half] scales
-template <int RT> constexpr int item_bytes = RT == 8 ? HBLK : RT / 16 * QBLK;  // RT: query rows an item
+constexpr int NRB = 2;                                 // blocks of 16 rows an item that is not one of 8
+template <int RT> constexpr int item_bytes = RT == 8 ? HBLK : NRB * QBLK;  // RT: query rows an item
 constexpr int WAVES = 4;
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -38,7 +39,7 @@ struct Kv4Args {
     const int32_t *past, *cu, *table, *slot, *seq;
     const float *qg, *k, *v, *wq, *wk;
     uint8_t *cache;
-    uint8_t *Q;                 // [nkv][items][rows / 16] query blocks of QBLK bytes
+    uint8_t *Q;                 // [nkv][items] query operands of item_bytes
     float *part_o;              // [items][nkv][nsplit][rows][HD]
     float *part_ml;             // [items][nkv][nsplit][rows][2]
     float *og;
@@ -77,13 +78,18 @@ __device__ __forceinline__ void sin_cos(double x, double &s, double &c) {
     if (q == 1 || q == 2) c = -c;
 }
 
-// One token: sines and cosines of its position, its keys and values into their page, its queries as operands.
-template <int RT>
-__global__ void __launch_bounds__(256, 2) k_kv4_prep(const Kv4Args a) {
+// One token: sines and cosines of its position, its keys and values into their page, its queries as operands.  A wave takes
+// one row of keys or values, or eight query heads.  What bounds it is the way through one token (a load, 64-bit sines, the
+// norm, five conversions one after the other): 6 us.  So a small batch gets workgroups for all of a token's tasks at once
+// (7.4 -> 6.4 us at one token of 2 + 2 + 16 heads, 9.0 -> 6.7 us at 64), and a large one two launches (PART 1: keys and
+// values, 2: queries): the keys' share in a kernel of its own has room for three times the waves.
+enum { PREP_ALL, PREP_KEYS, PREP_QUERIES };
+template <int RT, int PART>
+__global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(const Kv4Args a) {
     __shared__ double cs[MAXROT], sn[MAXROT];  // of each rotated dim; the sine with the sign that its pair's other value gets
     __shared__ float cf[MAXROT], sf[MAXROT];
-    __shared__ double krow[WAVES][MAXROT];
-    __shared__ float qrow[WAVES][8][MAXROT + 4];
+    __shared__ double krow[PART == PREP_QUERIES ? 1 : WAVES][MAXROT];
+    __shared__ float qrow[PART == PREP_KEYS ? 1 : WAVES][8][MAXROT + 4];
     const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int total = min(a.cu[a.B], a.T);
     if (t >= total) return;
@@ -92,12 +98,27 @@ __global__ void __launch_bounds__(256, 2) k_kv4_prep(const Kv4Args a) {
         if (threadIdx.x == 0) atomicOr(a.status, FN_STATUS_ROWS);
         return;
     }
+    // the wave's first rows are requested before anything that waits
+    const int waves = blockDim.x >> 6, octets = (a.nq + 7) / 8;
+    const int from = PART == PREP_QUERIES ? 2 * a.nkv : 0, tasks = 2 * a.nkv + (PART == PREP_KEYS ? 0 : octets);
+    const int first = from + wave + waves * blockIdx.y;
+    float4 row[8];
+    auto request = [&](int task) __attribute__((always_inline)) {
+        if (PART == PREP_KEYS || (PART == PREP_ALL && task < 2 * a.nkv)) {
+            row[0] = reinterpret_cast<const float4 *>((task & 1 ? a.v : a.k) + ((size_t) t * a.nkv + (task >> 1)) * HD)[lane];
+        } else {
+            const int h = min((task - 2 * a.nkv) * 8 + (lane >> 3), a.nq - 1);
+            const float4 *src = reinterpret_cast<const float4 *>(a.qg + ((size_t) t * a.nq + h) * 2 * HD + 32 * (lane & 7));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[i] = src[i];
+        }
+    };
+    if (first < tasks) request(first);
     const long long P = (long long) a.past[b] + (t - a.cu[b]);
     if ((a.past[b] < 0 || P >= (long long) a.mb * PG) && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_POS);
     const int half = a.nrot / 2;
     // the angle in 64 bits: a float product is off by up to half a radian at a million tokens
-    if (threadIdx.x < MAXROT) {
-        const int d = threadIdx.x;
+    for (int d = threadIdx.x; d < MAXROT; d += blockDim.x) {
         double sv = 0.0, cv = 1.0;
         if (d < a.nrot) sin_cos((double) P * a.freq[d < half ? d : d - half], sv, cv);
         if (d < half) sv = -sv;
@@ -107,16 +128,15 @@ __global__ void __launch_bounds__(256, 2) k_kv4_prep(const Kv4Args a) {
     __syncthreads();
     const int slot = a.slot[t];
     const bool put = slot >= 0 && slot / PG < a.npages;
-    if (slot >= 0 && !put && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_PAGE);
-    const int octets = (a.nq + 7) / 8;
-    for (int task = wave; task < 2 * a.nkv + octets; task += WAVES) {
-        if (task < 2 * a.nkv) {
+    if (PART != PREP_QUERIES && slot >= 0 && !put && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_PAGE);
+    for (int task = first; task < tasks; task += waves * gridDim.y) {
+        if (task != first) request(task);
+        if (PART == PREP_KEYS || (PART == PREP_ALL && task < 2 * a.nkv)) {
             if (!put) continue;
             const int g = task >> 1;
             uint8_t *page = a.cache + ((size_t) (slot / PG) * a.nkv + g) * HEAD_BYTES;
             const bool is_v = task & 1;
-            const float4 x = reinterpret_cast<const float4 *>((is_v ? a.v : a.k) + ((size_t) t * a.nkv + g) * HD)[lane];
-            double y[4] = {x.x, x.y, x.z, x.w};
+            double y[4] = {row[0].x, row[0].y, row[0].z, row[0].w};
             if (is_v) {
                 store_row<false>(page, slot % PG, y, lane, a.status);
                 continue;
@@ -148,13 +168,12 @@ __global__ void __launch_bounds__(256, 2) k_kv4_prep(const Kv4Args a) {
         // eight query heads a wave, a lane holds one 32-dim group of one
         const int h = (task - 2 * a.nkv) * 8 + (lane >> 3), gi = lane & 7;
         const bool on = h < a.nq;
-        const float4 *src = reinterpret_cast<const float4 *>(a.qg + ((size_t) t * a.nq + min(h, a.nq - 1)) * 2 * HD + 32 * gi);
         const float4 *wsrc = reinterpret_cast<const float4 *>(a.wq + 32 * gi);
         float x[32];
         float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float4 f = src[i];
+            const float4 f = row[i];
             x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
             ss += sumsq4(f);
         }
@@ -261,8 +280,25 @@ constexpr float SM_SCALE = 0.0625f * 1.4426950408889634f;  // 1 / sqrt(HD), and 
 constexpr float SLACK = 8.0f * 16.0f;                      // growth of a row's largest raw score that moves its reference
 constexpr float PUP = 16.0f;                               // probabilities times 2^16: the parts of the least ones stay normal
 
-// A 32-key block of one head in 49 registers.  A wave holds two; what it has used up it requests of the next block but one
-// at once (K behind the scores, V behind each pair of its groups), so that about one and a half blocks are in flight.
+// 64 dims of the lane's eight keys as bf16 pairs: dims 32 t + 2 (l % 16), + 1
+__device__ __forceinline__ void values_of(const v4u &v, const v4u &vs, int t, uint32_t (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t w = v[t * 2 + j / 4], s4 = vs[t * 2 + j / 4];
+        // the instruction takes the scale from bits 30:23 of a float and looks at no other
+        const float s = __uint_as_float(j % 4 == 3 ? s4 >> 1 : s4 << (23 - 8 * (j % 4)));
+        const auto cv = [&](auto sel) {
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, decltype(sel)::value));
+        };
+        x[j] = j % 4 == 0   ? cv(std::integral_constant<int, 0>{})
+               : j % 4 == 1 ? cv(std::integral_constant<int, 1>{})
+               : j % 4 == 2 ? cv(std::integral_constant<int, 2>{})
+                            : cv(std::integral_constant<int, 3>{});
+    }
+}
+
+// A 32-key block of one head in 49 registers.  What a wave has used up it requests of its next block at once (K behind the
+// scores, V behind each pair of its groups).
 struct KvBlock {
     v4u k[2][2];  // [16-key block][half of the row]
     uint32_t ks;
@@ -279,44 +315,32 @@ struct KvBlock {
         v[i] = *reinterpret_cast<const v4u *>(p + VC + kk * 4096 + i * 1024 + lane * 16);
         vs[i] = *reinterpret_cast<const v4u *>(p + VS + kk * 256 + i * 16 + (lane >> 4) * 64);
     }
-    // values of the lane's dims 32 t + 2 (l % 16), + 1 of its eight keys
-    __device__ __forceinline__ void values(int t, uint32_t (&x)[8]) const {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t w = v[t / 2][t % 2 * 2 + j / 4], s4 = vs[t / 2][t % 2 * 2 + j / 4];
-            // the instruction takes the scale from bits 30:23 of a float and looks at no other
-            const float s = __uint_as_float(j % 4 == 3 ? s4 >> 1 : s4 << (23 - 8 * (j % 4)));
-            const auto cv = [&](auto sel) {
-                return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, decltype(sel)::value));
-            };
-            x[j] = j % 4 == 0   ? cv(std::integral_constant<int, 0>{})
-                   : j % 4 == 1 ? cv(std::integral_constant<int, 1>{})
-                   : j % 4 == 2 ? cv(std::integral_constant<int, 2>{})
-                                : cv(std::integral_constant<int, 3>{});
-        }
-    }
+    __device__ __forceinline__ void values(int t, uint32_t (&x)[8]) const { values_of(v[t / 2], vs[t / 2], t % 2, x); }
 };
 
 // The state of one row (the lane's column) of an online softmax.  MASK: keys from lim on count for nothing.
 struct Softmax {
     float m = -INFINITY, l = 0.0f;
-    // eight raw scores (key + 16 (i / 4) + i % 4) -> probabilities 2^PUP p; returns the factor of what was summed before
-    template <bool MASK> __device__ __forceinline__ float step(const float (&s)[8], float (&p)[8], int key, int lim) {
-        float sc[8], mx = -INFINITY;
+    // eight raw scores (key + 16 (i / 4) + i % 4), those behind the mask -infinity; returns the largest of the lane's row
+    template <bool MASK> static __device__ __forceinline__ float largest(float (&s)[8], int key, int lim) {
+        float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            sc[i] = !MASK || key + 16 * (i / 4) + i % 4 < lim ? s[i] : -INFINITY;
-            mx = fmaxf(mx, sc[i]);
+            if (MASK) s[i] = key + 16 * (i / 4) + i % 4 < lim ? s[i] : -INFINITY;
+            mx = fmaxf(mx, s[i]);
         }
-        mx = max_quarters(mx);
+        return max_quarters(mx);
+    }
+    // -> probabilities 2^PUP p; returns the factor of what was summed before
+    template <bool MASK> __device__ __forceinline__ float step(const float (&s)[8], float mx, float (&p)[8]) {
         const bool first = m == -INFINITY, moved = !first && mx > m + SLACK;
         const float mn = first || moved ? mx : m;
         const float corr = moved ? __builtin_amdgcn_exp2f((m - mn) * SM_SCALE) : 1.0f;
         float ps = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i] - mn, SM_SCALE, PUP));
-            if (MASK && sc[i] == -INFINITY) p[i] = 0.0f;
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i] - mn, SM_SCALE, PUP));
+            if (MASK && s[i] == -INFINITY) p[i] = 0.0f;
             ps += p[i];
         }
         l = fmaf(l, corr, ps);
@@ -325,21 +349,17 @@ struct Softmax {
     }
 };
 
-// grid (nsplit, nkv, items), 256 threads: the RT rows of an item (8, 16 or 32) against the keys of a split; the waves take
-// 32-key blocks in turn, each with its own softmax state, and meet at the end.
-// Eight rows (a decode step of up to 8 query heads a kv head) use both halves of the products' 16 columns.  Scores:
+// grid (nsplit, nkv, items), four waves: the eight rows of an item (a decode step of up to 8 query heads a kv head) against
+// the keys of a split; the waves take 32-key blocks in turn, each with its own softmax state, and meet at the end.
+// Eight rows use both halves of the products' 16 columns.  Scores:
 // columns 0..7 take parts 0..2 of the queries and 8..15 parts 3, 4, so three products do for five, and a rotation by
 // eight lanes adds the halves.  P.V: the conversion leaves dims 2m, 2m + 1 of a key in one register, which as it stands
 // is two contraction slots; the columns 0..7 hold a probability in the first of them and 0 in the second, which gives
 // the even dims, and 8..15 the other way round.  So nothing is permuted and the sums take half the registers.
-template <int RT>
-__global__ void __launch_bounds__(WAVES * 64, RT == 32 ? 1 : RT == 16 ? 2 : 3) k_attn_kv4(const Kv4Args a) {
-    constexpr bool HALF = RT == 8;
-    constexpr int NRB = HALF ? 1 : RT / 16, NT = HALF ? 8 : 16;      // row blocks, output tiles a row block
-    constexpr int NB = 1;                                 // key blocks in registers
-    constexpr int DC = HALF ? 256 : 64, MS = DC + 4;                 // dims merged at a time, floats a row of the merge
-    constexpr int QB = item_bytes<RT>, MB = WAVES * RT * MS * 4;
-    __shared__ __align__(16) uint8_t lds[QB > MB ? QB : MB];
+__global__ void __launch_bounds__(WAVES * 64, 3) k_attn_kv4(const Kv4Args a) {
+    constexpr int RT = 8, MS = HD + 4;  // rows, floats a row of the merge
+    constexpr int MB = WAVES * RT * MS * 4;
+    __shared__ __align__(16) uint8_t lds[HBLK > MB ? HBLK : MB];
     __shared__ float wm[WAVES][RT], wl[WAVES][RT];
     const int sp = blockIdx.x, g = blockIdx.y, item = a.items - 1 - (int) blockIdx.z;  // the longest rows first
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -363,62 +383,44 @@ __global__ void __launch_bounds__(WAVES * 64, RT == 32 ? 1 : RT == 16 ? 2 : 3) k
     auto ok = [&](int page) { return page >= 0 && page < a.npages; };
     auto base_of = [&](int page) { return cache + (ok(page) ? page : 0) * stride; };  // in bounds; the block is passed over
     int kb = k0 / 32 + wave;
-    int page[NB + 1];  // of this block and the next ones
+    int page = page_of(kb), next = page_of(kb + WAVES);
+    KvBlock x;
+    if (kb * 32 < k1) {
+        const uint8_t *p = base_of(page);
+        x.load_k(p, kb & 1, lane);
 #pragma unroll
-    for (int i = 0; i <= NB; ++i) page[i] = page_of(kb + i * WAVES);
-    KvBlock x[NB];
-    auto load_all = [&](KvBlock &y, int at, int pg) __attribute__((always_inline)) {
-        const uint8_t *p = base_of(pg);
-        y.load_k(p, at & 1, lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y.load_v(i, p, at & 1, lane);
-    };
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-        if ((kb + i * WAVES) * 32 < k1) load_all(x[i], kb + i * WAVES, page[i]);
+        for (int i = 0; i < 4; ++i) x.load_v(i, p, kb & 1, lane);
+    }
     // the item's query operands into the LDS
-    const v4u *Q = reinterpret_cast<const v4u *>(a.Q + ((size_t) g * a.items + item) * item_bytes<RT>);
-    for (int i = threadIdx.x; i < QB / 16; i += WAVES * 64) reinterpret_cast<v4u *>(lds)[i] = Q[i];
+    const v4u *Q = reinterpret_cast<const v4u *>(a.Q + ((size_t) g * a.items + item) * HBLK);
+    for (int i = threadIdx.x; i < HBLK / 16; i += WAVES * 64) reinterpret_cast<v4u *>(lds)[i] = Q[i];
     __syncthreads();
     uint32_t hs[2];
-    v2u qs[NRB][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        if (HALF) hs[u] = *reinterpret_cast<const uint32_t *>(lds + 2 * HSLOT * FRAG + u * 256 + lane * 4);
-#pragma unroll
-        for (int j = 0; j < NRB; ++j)
-            if (!HALF) qs[j][u] = *reinterpret_cast<const v2u *>(lds + j * QBLK + 2 * NPART * FRAG + u * 512 + lane * 8);
-    }
+    for (int u = 0; u < 2; ++u) hs[u] = *reinterpret_cast<const uint32_t *>(lds + 2 * HSLOT * FRAG + u * 256 + lane * 4);
     auto operand = [&](int at) __attribute__((always_inline)) {
         const v4u qa = *reinterpret_cast<const v4u *>(lds + at + lane * 16);
         const v2u qb = *reinterpret_cast<const v2u *>(lds + at + 1024 + lane * 8);
         return v6u{qa[0], qa[1], qa[2], qa[3], qb[0], qb[1]};
     };
-    int lim[NRB];
+    const int lim = min(visible(min((r0 + (lane & 7)) / a.grp, n - 1)), k1);
+    v4f o[8];
+    Softmax sm;
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < NRB; ++j)
-        lim[j] = min(visible(min((r0 + 16 * j + (lane & (HALF ? 7 : 15))) / a.grp, n - 1)), k1);
-    v4f o[NRB][NT];
-    Softmax sm[NRB];
-#pragma unroll
-    for (int j = 0; j < NRB; ++j)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[j][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    auto block = [&](KvBlock &x) __attribute__((always_inline)) {
-        // what takes the place of this block: the NB-th after it (at the end, this one again)
-        const bool more = (kb + NB * WAVES) * 32 < k1;
-        const int here = page[0], kn = more ? kb + NB * WAVES : kb, pn = more ? page[NB] : here;
-        const uint8_t *p = base_of(pn);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) page[i] = page[i + 1];
-        page[NB] = page_of(kb + (NB + 1) * WAVES);
+    for (int t = 0; t < 8; ++t) o[t] = zero;
+    for (; kb * 32 < k1; kb += WAVES) {
+        // what takes the place of this block: the wave's next (at the end, this one again)
+        const bool more = (kb + WAVES) * 32 < k1;
+        const int here = page, kn = more ? kb + WAVES : kb;
+        page = more ? next : here;
+        const uint8_t *p = base_of(page);
+        next = page_of(kb + 2 * WAVES);
         const bool in = ok(here);  // a block outside the cache counts for nothing
         if (!in && lane == 0) atomicOr(a.status, FN_STATUS_PAGE);
         // scores, in two sums: what the first part of the queries gives, and the small rest
-        float S[NRB][8];
-        const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (HALF) {
-            v4f big[2] = {zero, zero}, small[2] = {zero, zero};
+        float S[8];
+        v4f big[2] = {zero, zero}, small[2] = {zero, zero};
 #define FN_KV4_SLOT(U, P)                                                                              \
     do {                                                                                              \
         const v6u q = operand(((U) * HSLOT + (P)) * FRAG);                                             \
@@ -426,19 +428,210 @@ __global__ void __launch_bounds__(WAVES * 64, RT == 32 ? 1 : RT == 16 ? 2 : 3) k
         acc[0] = mma_k<(U), (P)>(x.k[0][U], (int) x.ks, q, (int) hs[U], acc[0]);                       \
         acc[1] = mma_k<2 + (U), (P)>(x.k[1][U], (int) x.ks, q, (int) hs[U], acc[1]);                   \
     } while (0)
-            FN_KV4_SLOT(0, 1);
-            FN_KV4_SLOT(0, 0);
-            FN_KV4_SLOT(0, 2);
-            FN_KV4_SLOT(1, 0);
-            FN_KV4_SLOT(1, 1);
-            FN_KV4_SLOT(1, 2);
+        FN_KV4_SLOT(0, 1);
+        FN_KV4_SLOT(0, 0);
+        FN_KV4_SLOT(0, 2);
+        FN_KV4_SLOT(1, 0);
+        FN_KV4_SLOT(1, 1);
+        FN_KV4_SLOT(1, 2);
 #undef FN_KV4_SLOT
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float s = big[i / 4][i % 4] + small[i / 4][i % 4];
-                S[0][i] = s + dpp_ror<8>(s);
+        for (int i = 0; i < 8; ++i) {
+            const float s = big[i / 4][i % 4] + small[i / 4][i % 4];
+            S[i] = s + dpp_ror<8>(s);
+        }
+        x.load_k(p, kn & 1, lane);
+        if (!in || kb * 32 + 32 > kvalid) {  // rows of the page that hold no token: their value scales may be anything
+            const int at = kb * 32 + 4 * (lane >> 4), end = in ? kvalid : 0;
+            uint32_t keep[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) keep[j / 4] |= at + 16 * (j / 4) + j % 4 < end ? 0xffu << (8 * (j % 4)) : 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.vs[i] &= v4u{keep[0], keep[1], keep[0], keep[1]};
+        }
+        float pr[8];
+        const int key = kb * 32 + 4 * (lane >> 4);
+        const float corr = in && kb * 32 + 32 <= all ? sm.step<false>(S, Softmax::largest<false>(S, key, lim), pr)
+                                                     : sm.step<true>(S, Softmax::largest<true>(S, key, in ? lim : 0), pr);
+        if (__ballot(corr != 1.0f)) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) o[t] *= corr;
+        }
+        // o += V^T P^T, 32 dims at a time, the probabilities in three bf16 parts
+        v4u P[2][3];  // [16-key block][part]; parts by truncation (8 bits each: exact), in the half of the register that
+                      // the column takes
+        const int sh = lane & 8 ? 0 : 16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float f = pr[i];
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                const uint32_t h = __float_as_uint(f) & 0xffff0000u;
+                P[i / 4][q][i % 4] = h >> sh;
+                f -= __uint_as_float(h);
             }
+        }
+        uint32_t w[2][8];
+        x.values(0, w[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {  // the next 32 dims are converted between the products
+            if (t < 7) x.values(t + 1, w[(t + 1) & 1]);
+            if (t % 2 == 0 && t < 6) x.load_v(t / 2, p, kn & 1, lane);
+            if (t == 7) x.load_v(3, p, kn & 1, lane);
+#pragma unroll
+            for (int q = 2; q >= 0; --q)
+#pragma unroll
+                for (int hb = 0; hb < 2; ++hb) {
+                    const uint32_t *y = w[t & 1] + 4 * hb;
+                    o[t] = mma_v(v4u{y[0], y[1], y[2], y[3]}, P[hb][q], o[t]);
+                }
+#pragma unroll
+            for (int i = 0; i < 6; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // the waves meet: reference of every row, then the sums
+    const float ls = sum_quarters(sm.l);
+    if (lane < RT) {
+        wm[wave][lane] = sm.m;
+        wl[wave][lane] = ls;
+    }
+    float *mo = reinterpret_cast<float *>(lds);
+    __syncthreads();  // the query operands have been read
+    float *d0 = mo + (wave * RT + (lane & 7)) * MS + 8 * (lane >> 4) + ((lane >> 3) & 1);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d0[32 * t + 2 * i] = o[t][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < RT * HD / 4; i += WAVES * 64) {
+        const int row = i / (HD / 4), r = r0 + row, d = i % (HD / 4) * 4;
+        if (r >= rows) continue;
+        float M = wm[0][row];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) M = fmaxf(M, wm[w][row]);
+        float L = 0.0f;
+        float4 s = f4(0.0f);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float mw = wm[w][row];
+            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - M) * SM_SCALE);
+            L = fmaf(wl[w][row], f, L);
+            s = add_scaled(s, *reinterpret_cast<const float4 *>(mo + (w * RT + row) * MS + d), f);
+        }
+        if (a.nsplit == 1) {
+            const int t = r / a.grp;
+            const size_t at = (size_t) (c0 + t) * a.nq + g * a.grp + (r - t * a.grp);
+            const float4 z = *reinterpret_cast<const float4 *>(a.qg + (at * 2 + 1) * HD + d);
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees no key: zeros
+            *reinterpret_cast<float4 *>(a.og + at * HD + d) =
+                make_float4(s.x * inv * sigmoidf_(z.x), s.y * inv * sigmoidf_(z.y), s.z * inv * sigmoidf_(z.z),
+                            s.w * inv * sigmoidf_(z.w));
         } else {
+            const size_t at = (((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + row;
+            *reinterpret_cast<float4 *>(a.part_o + at * HD + d) = s;
+            if (d == 0) {
+                a.part_ml[2 * at] = M;
+                a.part_ml[2 * at + 1] = L;
+            }
+        }
+    }
+}
+
+// grid (nsplit, nkv, items), four waves: the 32 rows of an item against the keys of a split, 128 keys at a time.  For the
+// scores a wave takes 32 of the keys, for the values a quarter of the dims: so each value is converted once for all rows,
+// the sums of a wave are 32 registers and not 128 (which left one wave a SIMD: 463 us for what now takes 340), and nothing
+// is left to be joined at the end.  The waves share the rows' references (a row's largest score goes through the LDS) and
+// the probabilities.
+// What bounds it: 136 matrix instructions of 16 cycles and some 600 vector instructions of 4 a wave and step, which two
+// waves a SIMD overlap in part, and 240 KB a step through the LDS.  A prompt of 4001 tokens, 16 + 2 heads: 340 us, the
+// matrix instructions alone 113 us; 24 requests of 1 to 300 tokens over up to 8k keys: 683 us, 329 us.
+__global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a) {
+    constexpr int RT = 16 * NRB, STEP = WAVES * 32;
+    __shared__ __align__(16) uint8_t lq[NRB * QBLK];
+    __shared__ v4u lp[WAVES][NRB][3][64];  // probabilities of 32 keys: [row block][part]
+    __shared__ float lm[WAVES][RT], ll[WAVES][RT];
+    const int sp = blockIdx.x, g = blockIdx.y, item = a.items - 1 - (int) blockIdx.z;  // the longest rows first
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15;
+    const int b = request_of(a.cu, a.B, item, a.grp, RT);
+    const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r0 = (item - first_item(a.cu, b, a.grp, RT)) * RT;
+    const int rows = n * a.grp;
+    if (c0 < 0 || r0 < 0 || r0 >= rows) return;
+    const int past = a.past[b], cap = a.mb * PG;
+    auto visible = [&](int t) { return past < 0 ? 0 : (int) min((long long) past + t + 1, (long long) cap); };
+    const int kvalid = visible(n - 1), kmax = visible((min(r0 + RT, rows) - 1) / a.grp);
+    const int tiles = (kmax + PG - 1) / PG, per = (tiles + a.nsplit - 1) / a.nsplit;
+    const int k0 = min(sp * per, tiles) * PG, k1 = min(min((sp + 1) * per, tiles) * PG, kmax);
+    const int all = min(visible(r0 / a.grp), k1);  // keys that every row of the item sees
+
+    // through the scalar cache: a vector load's wait would wait for every key block in flight, too
+    typedef const __attribute__((address_space(4))) int32_t *scalar_i32;
+    const scalar_i32 table = (scalar_i32) (uintptr_t) (a.table + (size_t) b * a.mb);
+    const size_t stride = (size_t) a.nkv * HEAD_BYTES;
+    const uint8_t *cache = a.cache + (size_t) g * HEAD_BYTES;
+    auto page_of = [&](int k) { return k < k1 ? table[k / PG] : -1; };
+    auto ok = [&](int page) { return page >= 0 && page < a.npages; };
+    auto base_of = [&](int page) { return cache + (ok(page) ? page : 0) * stride; };  // in bounds; the block is passed over
+    int page[2] = {page_of(k0), page_of(k0 + PG)}, next[2] = {page_of(k0 + STEP), page_of(k0 + STEP + PG)};
+    v4u k[2][2], v[WAVES], vs[WAVES];  // keys of the wave's 32: [16][half of the row]; its dims of each 32 keys
+    uint32_t ks;
+    auto load_k = [&](const int (&pg)[2]) __attribute__((always_inline)) {
+        const uint8_t *p = base_of(wave < 2 ? pg[0] : pg[1]);
+        const int kk = wave & 1;
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) k[hb][u] = *reinterpret_cast<const v4u *>(p + kk * 4096 + (hb * 2 + u) * 1024 + lane * 16);
+        ks = *reinterpret_cast<const uint32_t *>(p + KS + kk * 256 + lane * 4);
+    };
+    auto load_v = [&](int c, const int (&pg)[2]) __attribute__((always_inline)) {
+        const uint8_t *p = base_of(pg[c / 2]);
+        v[c] = *reinterpret_cast<const v4u *>(p + VC + c % 2 * 4096 + wave * 1024 + lane * 16);
+        vs[c] = *reinterpret_cast<const v4u *>(p + VS + c % 2 * 256 + wave * 16 + (lane >> 4) * 64);
+    };
+    // in the order of the loop's requests: its waits count them as both ways into it have them
+    load_k(page);
+#pragma unroll
+    for (int c = 0; c < WAVES; ++c) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(c, page);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // the item's query operands into the LDS
+    const v4u *Q = reinterpret_cast<const v4u *>(a.Q + ((size_t) g * a.items + item) * item_bytes<RT>);
+    for (int i = threadIdx.x; i < NRB * QBLK / 16; i += WAVES * 64) reinterpret_cast<v4u *>(lq)[i] = Q[i];
+    __syncthreads();
+    v2u qs[NRB][2];
+    int lim[NRB];
+    v4f o[NRB][2][2];  // [32 dims of the wave's 64][even, odd]: lane = row, dims 8 (lane / 16) + 2 i
+    Softmax sm[NRB];
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NRB; ++j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            qs[j][u] = *reinterpret_cast<const v2u *>(lq + j * QBLK + 2 * NPART * FRAG + u * 512 + lane * 8);
+            o[j][u][0] = o[j][u][1] = zero;
+        }
+        lim[j] = min(visible(min((r0 + 16 * j + col) / a.grp, n - 1)), k1);
+    }
+    auto operand = [&](int at) __attribute__((always_inline)) {
+        const v4u qa = *reinterpret_cast<const v4u *>(lq + at + lane * 16);
+        const v2u qb = *reinterpret_cast<const v2u *>(lq + at + 1024 + lane * 8);
+        return v6u{qa[0], qa[1], qa[2], qa[3], qb[0], qb[1]};
+    };
+    for (int at = k0; at < k1; at += STEP) {
+        const int kb = at + 32 * wave;  // the wave's first key
+        const int own = wave < 2 ? page[0] : page[1];
+        const bool in = kb < k1 && ok(own);  // a block outside the cache counts for nothing
+        if (kb < k1 && !in && lane == 0) atomicOr(a.status, FN_STATUS_PAGE);
+        // scores, in two sums: what the first part of the queries gives, and the small rest
+        float S[NRB][8];
+        {
             v4f big[2][NRB], small[2][NRB];
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb)
@@ -449,8 +642,8 @@ __global__ void __launch_bounds__(WAVES * 64, RT == 32 ? 1 : RT == 16 ? 2 : 3) k
         _Pragma("unroll") for (int j = 0; j < NRB; ++j) {                                                            \
             const v6u q = operand(j * QBLK + ((U) * NPART + (P)) * FRAG);                                            \
             v4f(&acc)[2][NRB] = (P) == 0 ? big : small;                                                              \
-            acc[0][j] = mma_k<(U), (P) % 4>(x.k[0][U], (int) x.ks, q, (int) qs[j][U][(P) / 4], acc[0][j]);           \
-            acc[1][j] = mma_k<2 + (U), (P) % 4>(x.k[1][U], (int) x.ks, q, (int) qs[j][U][(P) / 4], acc[1][j]);       \
+            acc[0][j] = mma_k<(U), (P) % 4>(k[0][U], (int) ks, q, (int) qs[j][U][(P) / 4], acc[0][j]);               \
+            acc[1][j] = mma_k<2 + (U), (P) % 4>(k[1][U], (int) ks, q, (int) qs[j][U][(P) / 4], acc[1][j]);           \
         }                                                                                                           \
     } while (0)
             FN_KV4_PART(0, 0);
@@ -469,186 +662,140 @@ __global__ void __launch_bounds__(WAVES * 64, RT == 32 ? 1 : RT == 16 ? 2 : 3) k
 #pragma unroll
                 for (int i = 0; i < 8; ++i) S[j][i] = big[i / 4][j][i % 4] + small[i / 4][j][i % 4];
         }
-        x.load_k(p, kn & 1, lane);
-        if (!in || kb * 32 + 32 > kvalid) {  // rows of the page that hold no token: their value scales may be anything
-            const int at = kb * 32 + 4 * (lane >> 4), end = in ? kvalid : 0;
-            uint32_t keep[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) keep[j / 4] |= at + 16 * (j / 4) + j % 4 < end ? 0xffu << (8 * (j % 4)) : 0u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.vs[i] &= v4u{keep[0], keep[1], keep[0], keep[1]};
-        }
-        float pr[NRB][8], corr[NRB];
-        bool moved = false;
-        const int key = kb * 32 + 4 * (lane >> 4);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool whole = in && kb + 32 <= all;
+        const int key = kb + 4 * (lane >> 4);
 #pragma unroll
         for (int j = 0; j < NRB; ++j) {
-            corr[j] = in && kb * 32 + 32 <= all ? sm[j].template step<false>(S[j], pr[j], key, lim[j])
-                                                : sm[j].template step<true>(S[j], pr[j], key, in ? lim[j] : 0);
+            const float mx = whole ? Softmax::largest<false>(S[j], key, lim[j]) : Softmax::largest<true>(S[j], key, in ? lim[j] : 0);
+            if (lane < 16) lm[wave][16 * j + lane] = mx;
+        }
+        lds_barrier();  // the largest scores are there, and the last probabilities have been read
+        bool moved = false;
+        float corr[NRB];
+#pragma unroll
+        for (int j = 0; j < NRB; ++j) {
+            float p[8];
+            const float mx = fmaxf(fmaxf(lm[0][16 * j + col], lm[1][16 * j + col]), fmaxf(lm[2][16 * j + col], lm[3][16 * j + col]));
+            corr[j] = whole ? sm[j].template step<false>(S[j], mx, p) : sm[j].template step<true>(S[j], mx, p);
             moved |= corr[j] != 1.0f;
+            v4u parts[3];  // three bf16 parts of each
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float f = p[2 * i], h = p[2 * i + 1];
+#pragma unroll
+                for (int q = 0; q < 3; ++q) {
+                    const uint32_t w = bf16_pair(f, h);
+                    parts[q][i] = w;
+                    f -= __uint_as_float(w << 16);
+                    h -= __uint_as_float(w & 0xffff0000u);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 3; ++q) lp[wave][j][q][lane] = parts[q];
         }
         if (__ballot(moved)) {
 #pragma unroll
             for (int j = 0; j < NRB; ++j)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) o[j][t] *= corr[j];
+                for (int t = 0; t < 4; ++t) o[j][t / 2][t % 2] *= corr[j];
         }
-        // o += V^T P^T, 32 dims at a time, the probabilities in three bf16 parts
-        if constexpr (HALF) {
-            v4u P[2][3];  // [16-key block][part]; parts by truncation (8 bits each: exact), in the half of the register that
-                          // the column takes
-            const int sh = lane & 8 ? 0 : 16;
+        // o += V^T P^T, 32 keys and 32 dims at a time; the next ones are converted between the products
+        v4u ve[2], vo[2];  // one dim of two keys
+        auto values = [&](int s) __attribute__((always_inline)) {
+            const int c = s / 2;
+            if (s % 2 == 0) {
+                const int kc = at + 32 * c;
+                const bool vin = kc < k1 && ok(page[c / 2]);
+                if (!vin || kc + 32 > kvalid) {  // rows of the page that hold no token: their scales may be anything
+                    const int first = kc + 4 * (lane >> 4), end = vin ? kvalid : 0;
+                    uint32_t keep[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float f = pr[0][i];
-#pragma unroll
-                for (int q = 0; q < 3; ++q) {
-                    const uint32_t h = __float_as_uint(f) & 0xffff0000u;
-                    P[i / 4][q][i % 4] = h >> sh;
-                    f -= __uint_as_float(h);
+                    for (int j = 0; j < 8; ++j)
+                        keep[j / 4] |= first + 16 * (j / 4) + j % 4 < end ? 0xffu << (8 * (j % 4)) : 0u;
+                    vs[c] &= v4u{keep[0], keep[1], keep[0], keep[1]};
                 }
             }
-            uint32_t w[2][8];
-            x.values(0, w[0]);
-            __builtin_amdgcn_sched_barrier(0);
+            uint32_t w[8];
+            values_of(v[c], vs[c], s % 2, w);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {  // the next 32 dims are converted between the products
-                if (t < 7) x.values(t + 1, w[(t + 1) & 1]);
-                if (t % 2 == 0 && t < 6) x.load_v(t / 2, p, kn & 1, lane);
-                if (t == 7) x.load_v(3, p, kn & 1, lane);
-#pragma unroll
-                for (int q = 2; q >= 0; --q)
-#pragma unroll
-                    for (int hb = 0; hb < 2; ++hb) {
-                        const uint32_t *y = w[t & 1] + 4 * hb;
-                        o[0][t] = mma_v(v4u{y[0], y[1], y[2], y[3]}, P[hb][q], o[0][t]);
-                    }
-#pragma unroll
-                for (int i = 0; i < 6; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < 4; ++i) {
+                ve[s & 1][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+                vo[s & 1][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
             }
-        } else {
-            v4u P[NRB][3];
+        };
+        values(0);
+        lds_barrier();  // the probabilities are there
+        v4u P[2][NRB][3];
+        auto load_p = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NRB; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float f = pr[j][2 * i], h = pr[j][2 * i + 1];
+                for (int q = 0; q < 3; ++q) P[c & 1][j][q] = lp[c][j][q][lane];
+        };
+        load_p(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                        const uint32_t w = bf16_pair(f, h);
-                        P[j][q][i] = w;
-                        f -= __uint_as_float(w << 16);
-                        h -= __uint_as_float(w & 0xffff0000u);
-                    }
+        for (int s = 0; s < 2 * WAVES; ++s) {
+            const int c = s / 2, t = s % 2;
+            if (s + 1 < 2 * WAVES) values(s + 1);
+            if (t == 0 && c + 1 < WAVES) load_p(c + 1);
+            if (t == 1 || s + 1 == 2 * WAVES) load_v(c, next);
+#pragma unroll
+            for (int q = 2; q >= 0; --q)
+#pragma unroll
+                for (int j = 0; j < NRB; ++j) {
+                    o[j][t][0] = mma_v(ve[s & 1], P[c & 1][j][q], o[j][t][0]);
+                    o[j][t][1] = mma_v(vo[s & 1], P[c & 1][j][q], o[j][t][1]);
                 }
-            v4u ve[2], vo[2];  // one dim of two keys
-            auto values = [&](int t) __attribute__((always_inline)) {
-                uint32_t w[8];
-                x.values(t, w);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    ve[t & 1][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
-                    vo[t & 1][i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
-                }
-            };
-            values(0);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                if (t < 7) values(t + 1);
-                if (t % 2 == 0 && t < 6) x.load_v(t / 2, p, kn & 1, lane);
-                if (t == 7) x.load_v(3, p, kn & 1, lane);
-#pragma unroll
-                for (int q = 2; q >= 0; --q)
-#pragma unroll
-                    for (int j = 0; j < NRB; ++j) {
-                        o[j][2 * t] = mma_v(ve[t & 1], P[j][q], o[j][2 * t]);
-                        o[j][2 * t + 1] = mma_v(vo[t & 1], P[j][q], o[j][2 * t + 1]);
-                    }
-#pragma unroll
-                for (int i = 0; i < 6 * NRB; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x2, 4 / NRB, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < 6 * NRB; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 4 / NRB, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-    };
-    while (kb * 32 < k1) {
-        block(x[0]);
-        kb += WAVES;
-        if (NB > 1) {
-            if (kb * 32 >= k1) break;
-            block(x[NB - 1]);
-            kb += WAVES;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            page[i] = next[i];
+            next[i] = page_of(at + 2 * STEP + PG * i);
         }
     }
-    // the waves meet: reference of every row, then the sums, DC dims at a time
+    // the rows' sums; the references are the same in all waves
 #pragma unroll
     for (int j = 0; j < NRB; ++j) {
         const float ls = sum_quarters(sm[j].l);
-        if (lane < (HALF ? 8 : 16)) {
-            wm[wave][16 * j + lane] = sm[j].m;
-            wl[wave][16 * j + lane] = ls;
-        }
+        if (lane < 16) ll[wave][16 * j + lane] = ls;
     }
-    float *mo = reinterpret_cast<float *>(lds);
+    __syncthreads();
 #pragma unroll
-    for (int c = 0; c < HD / DC; ++c) {
-        __syncthreads();  // the query operands, or the last dims, have been read
-        if constexpr (HALF) {
-            float *d = mo + (wave * RT + (lane & 7)) * MS + 8 * (lane >> 4) + ((lane >> 3) & 1);
+    for (int j = 0; j < NRB; ++j) {
+        const int row = 16 * j + col, r = r0 + row;
+        if (r >= rows) continue;
+        const float L = (ll[0][row] + ll[1][row]) + (ll[2][row] + ll[3][row]);
+        const int tok = r / a.grp, d = 64 * wave + 8 * (lane >> 4);
+        const size_t out = (size_t) (c0 + tok) * a.nq + g * a.grp + (r - tok * a.grp);
+        const size_t part = (((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + row;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees no key: zeros
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d[32 * t + 2 * i] = o[0][t][i];
-        } else {
-#pragma unroll
-            for (int j = 0; j < NRB; ++j)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {  // the lane's row, dims 8 (lane / 16) .. + 7 of the group
-                    float *d = mo + (wave * RT + 16 * j + (lane & 15)) * MS + 32 * t + 8 * (lane >> 4);
-                    const v4f e = o[j][4 * c + 2 * t], f = o[j][4 * c + 2 * t + 1];
-                    *reinterpret_cast<float4 *>(d) = make_float4(e[0], f[0], e[1], f[1]);
-                    *reinterpret_cast<float4 *>(d + 4) = make_float4(e[2], f[2], e[3], f[3]);
-                }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < RT * DC / 4; i += WAVES * 64) {
-            const int row = i / (DC / 4), r = r0 + row, d = i % (DC / 4) * 4;
-            if (r >= rows) continue;
-            float M = wm[0][row];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) M = fmaxf(M, wm[w][row]);
-            float L = 0.0f;
-            float4 s = f4(0.0f);
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                const float mw = wm[w][row];
-                const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - M) * SM_SCALE);
-                L = fmaf(wl[w][row], f, L);
-                s = add_scaled(s, *reinterpret_cast<const float4 *>(mo + (w * RT + row) * MS + d), f);
-            }
+        for (int t = 0; t < 4; ++t) {  // four dims
+            const v4f e = o[j][t / 2][0], f = o[j][t / 2][1];
+            const int i = t % 2 * 2, dim = d + 32 * (t / 2) + 4 * (t % 2);
+            const float4 x = make_float4(e[i], f[i], e[i + 1], f[i + 1]);
             if (a.nsplit == 1) {
-                const int t = r / a.grp;
-                const size_t at = (size_t) (c0 + t) * a.nq + g * a.grp + (r - t * a.grp);
-                const float4 z = *reinterpret_cast<const float4 *>(a.qg + (at * 2 + 1) * HD + DC * c + d);
-                const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees no key: zeros
-                *reinterpret_cast<float4 *>(a.og + at * HD + DC * c + d) =
-                    make_float4(s.x * inv * sigmoidf_(z.x), s.y * inv * sigmoidf_(z.y), s.z * inv * sigmoidf_(z.z),
-                                s.w * inv * sigmoidf_(z.w));
+                const float4 z = *reinterpret_cast<const float4 *>(a.qg + (out * 2 + 1) * HD + dim);
+                *reinterpret_cast<float4 *>(a.og + out * HD + dim) =
+                    make_float4(x.x * inv * sigmoidf_(z.x), x.y * inv * sigmoidf_(z.y), x.z * inv * sigmoidf_(z.z),
+                                x.w * inv * sigmoidf_(z.w));
             } else {
-                const size_t at = (((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + row;
-                *reinterpret_cast<float4 *>(a.part_o + at * HD + DC * c + d) = s;
-                if (c == 0 && d == 0) {
-                    a.part_ml[2 * at] = M;
-                    a.part_ml[2 * at + 1] = L;
-                }
+                *reinterpret_cast<float4 *>(a.part_o + part * HD + dim) = x;
             }
+        }
+        if (a.nsplit > 1 && wave == 0 && lane < 16) {
+            a.part_ml[2 * part] = sm[j].m;
+            a.part_ml[2 * part + 1] = L;
         }
     }
 }
@@ -695,17 +842,24 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
 }
 
 template <int RT> void launch(const Kv4Args &a, hipStream_t st) {
-    hipLaunchKernelGGL(k_kv4_prep<RT>, dim3(a.T), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_attn_kv4<RT>, dim3(a.nsplit, a.nkv, a.items), dim3(WAVES * 64), 0, st, a);
+    const int octets = (a.nq + 7) / 8, groups = (2 * a.nkv + octets + WAVES - 1) / WAVES;
+    if ((long long) a.T * groups <= 2 * device_cus()) {  // one round
+        hipLaunchKernelGGL((k_kv4_prep<RT, PREP_ALL>), dim3(a.T, groups), dim3(256), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((k_kv4_prep<8, PREP_KEYS>), dim3(a.T), dim3(64 * std::min(2 * a.nkv, WAVES)), 0, st, a);
+        hipLaunchKernelGGL((k_kv4_prep<RT, PREP_QUERIES>), dim3(a.T), dim3(64 * std::min(octets, WAVES)), 0, st, a);
+    }
+    hipLaunchKernelGGL(RT == 8 ? k_attn_kv4 : k_attn_kv4_rows, dim3(a.nsplit, a.nkv, a.items), dim3(WAVES * 64), 0, st, a);
     if (a.nsplit > 1) hipLaunchKernelGGL(k_kv4_combine<RT>, dim3(a.items * RT, a.nkv), dim3(256), 0, st, a);
 }
 
-// Query rows an item: what an average request has, up to 32.
-int item_rows(int B, int T, int grp) {
-    const long long rows = (long long) T * grp;
-    return rows <= 8ll * B ? 8 : rows <= 16ll * B ? 16 : 32;
-}
-size_t query_bytes(int rt) { return rt == 8 ? HBLK : rt * 1024; }
+// Query rows an item.  A request of up to 24 rows is cheaper as up to three items of eight, which read its keys one behind
+// the other, than as one of 32 in which rows are left empty.  8 query heads a kv head, 8k keys, us with 8 | 32 rows an item:
+// 16 requests of 1, 2, 3, 4 tokens 51 | 56, 51 | 56, 65 | 58, 72 | 62; 64 requests of 1, 2, 3 tokens 131 | 146, 158 | 184,
+// 172 | 182; 24 requests, 4 kv heads, 20k keys, of 1, 2, 3 tokens 195 | 218, 197 | 217, 218 | 299.  (16 rows an item won
+// by 9% at one of these and lost at the others.)
+int item_rows(int B, int T, int grp) { return (long long) T * grp <= 24ll * B ? 8 : 32; }
+size_t query_bytes(int rt) { return rt == 8 ? item_bytes<8> : item_bytes<32>; }
 
 }  // namespace
 
@@ -717,9 +871,13 @@ size_t kv4_work_bytes(int B, int T, int nq, int nkv, int hd, int nsplit) {
 
 int kv4_pick_nsplit(int B, int T, int nq, int nkv, int ctx) {
     const int grp = nq / nkv, rt = item_rows(B, T, grp);
-    const long long groups = std::max<long long>(B, ((long long) T * grp + rt - 1) / rt) * nkv;
-    const int most = std::max(1, (ctx + 127) / 128);  // a 32-key block for each wave
+    // one round of workgroups, two a CU: items of an average request times requests
+    const long long avg = ((long long) T * grp + B - 1) / B, groups = std::max(1ll, (avg + rt - 1) / rt) * B * nkv;
     const long long want = std::max(1ll, 2ll * device_cus() / groups);
+    // A split costs a row of sums that is written and read again, so the time is about u keys / nsplit + w nsplit, least at
+    // a multiple of sqrt(keys).  One token, 2 kv heads, us at 16, 32, 64, 128, 256 splits: 4k keys 25.0, 24.1, 24.7, 27.0,
+    // 32.6; 32k keys 43.4, 34.4, 30.6, 32.2, 38.9; 100k keys 86.5, 58.4, 45.4, 45.0, 52.1.
+    const int most = std::max(1, (int) (std::sqrt((double) ctx) * 0.5));
     return (int) std::min<long long>(want, most);
 }
 
@@ -741,7 +899,7 @@ int kv4_attn_launch(const Kv4Attn &p, hipStream_t st) {
     const int grp = p.nq / p.nkv, rt = item_rows(p.B, p.T, grp);
     if ((long long) p.T * grp > INT_MAX - 64) FN_FAIL("attn_kv4: too many query rows");
     const size_t items = item_count(p.B, p.T, grp, rt);
-    if (p.nkv > 65535 || items > 65535) FN_FAIL("attn_kv4: batch too large (at most 65535 requests and pieces of 32 query rows)");
+    if (p.nkv > 65535 || items > 65535) FN_FAIL("attn_kv4: batch too large (at most 65535 requests and pieces of their query rows)");
     if (p.work_bytes < kv4_work_bytes(p.B, p.T, p.nq, p.nkv, p.hd, p.nsplit)) FN_FAIL("attn_kv4: workspace too small");
     Kv4Args a{};
     a.B = p.B; a.T = p.T; a.nq = p.nq; a.nkv = p.nkv; a.grp = grp; a.mb = p.max_blocks; a.npages = p.npages;
@@ -754,7 +912,6 @@ int kv4_attn_launch(const Kv4Attn &p, hipStream_t st) {
     a.part_ml = a.part_o + items * p.nkv * rt * p.nsplit * HD;
     for (int i = 0; i < p.nrot / 2; ++i) a.freq[i] = std::pow((double) p.theta, -(2.0 * i) / p.nrot);
     if (rt == 8) launch<8>(a, st);
-    else if (rt == 16) launch<16>(a, st);
     else launch<32>(a, st);
     FN_CK(hipGetLastError());
     return 0;
