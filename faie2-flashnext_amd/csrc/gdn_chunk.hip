@@ -12,7 +12,7 @@
 //   k_chunk_scan, one a (request, value head, columns of S), which walks the request's chunks with its columns of S in
 //     registers: three small products one after the other a chunk, and two exchanges through the LDS.
 // W and U0 are formed before the scan, not M inside it: the scan is the sequential part, and M there is one more product
-// and exchange a chunk (15k tokens, 32 value heads: scan 596 us with M, 405 us with W; the other kernel 252 and 332 us).
+// and exchange a chunk (15k tokens, 32 value heads: scan 596 us with M, 405 us with W; the other kernel 252 and 278 us).
 // Products: an fp32 operand is two f16 values (hi and lo, 11 bits each) under a power-of-two scale, and a product is hi
 // hi + hi lo + lo hi on v_mfma_f32_16x16x32_f16: what is left out is 2^-22 of a product at the worst and 2^-24 in the
 // mean, in half the instructions of six bf16 products and a fifth of the time of fp32 ones.  f16's range is met by
@@ -82,7 +82,9 @@ __device__ __forceinline__ float silu_(float x) { return x * __builtin_amdgcn_rc
 __device__ __forceinline__ float4 lds4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 
 // grid (chunks, nkh), four waves.  What bounds it: memory.  15k tokens, 16 key and 32 value heads: 0.49 GB of q, k, v in,
-// 0.86 GB of operands out in 332 us, 4.1 TB/s.  M = (I + A)^-1 by blocks of 16: a wave inverts its diagonal block by
+// 0.86 GB of operands out in 278 us, 4.9 TB/s (all rows are requested before the first is waited for, and V and the gates
+// a part ahead: 332 us without).  In the block form, 4k tokens, 16 and 48 heads: 0.49 GB in 149 us, 3.2 TB/s; it uses all
+// 256 registers, and a chunk's three value heads one after the other leave two rounds of workgroups.  M = (I + A)^-1 by blocks of 16: a wave inverts its diagonal block by
 // substitution, one column a lane, and forms its block row from the diagonal leftwards on fp32 matrix instructions.
 template <bool BLOCK>
 __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
@@ -93,49 +95,62 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
     __shared__ double G[C];
     const GdnChunk &p = a.p;
     const int item = blockIdx.x, kh = blockIdx.y;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q4 = lane >> 4;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    int r = lane & 15, q4 = lane >> 4;
     const int b = request_of(p.cu, p.B, item, 1, C);
     const int c0 = p.cu[b], t0 = (item - first_item(p.cu, b, 1, C)) * C, n = min(C, min(p.cu[b + 1], p.T) - c0 - t0);
     if (c0 < 0 || t0 < 0 || n <= 0) return;
     const size_t row0 = (size_t) c0 + t0;
     uint8_t *kd = a.keys + ((size_t) item * p.nkh + kh) * KEY_BYTES;
 
+    const int per = p.nvh / p.nkh, Cc = 2 * p.nkh * D + p.nvh * D;
+    auto head_of = [&](int i) { return p.head_map == 0 ? kh + i * p.nkh : kh * per + i; };
+    float gate[2];  // beta, g of a head (of the block: what they are made from), a head ahead
+    auto request_gates = [&](int i) __attribute__((always_inline)) {
+        const size_t t = row0 + min(lane, n - 1), h = head_of(i);
+        gate[0] = BLOCK ? p.ab[t * 2 * p.nvh + p.nvh + h] : p.beta[t * p.nvh + h];
+        gate[1] = BLOCK ? p.ab[t * 2 * p.nvh + h] : p.g[t * p.nvh + h];
+    };
+    request_gates(0);
     // 1. q, k rows
     if (BLOCK) {
-        const int ch = tid & (D - 1), part = tid >> 7, Cc = 2 * p.nkh * D + p.nvh * D, col = (part * p.nkh + kh) * D + ch;
+        const int ch = tid & (D - 1), part = tid >> 7, col = (part * p.nkh + kh) * D + ch;
         const float4 w = *reinterpret_cast<const float4 *>(p.conv_w + 4 * col);
         const float *x = p.qkv + row0 * Cc + col;
-        float h[3];
+        const brsrc rd = buf(p.qkv + row0 * Cc, (uint32_t) n * Cc * 4);  // rows behind: 0
+        float h[3], v[C];
+#pragma unroll
+        for (int t = 0; t < C; ++t) v[t] = bld(rd, (uint32_t) (t * Cc + col) * 4, 0);
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
             const int t = t0 - 3 + j;
             h[j] = t >= 0 ? x[(ptrdiff_t) (j - 3) * Cc]
                           : p.conv_ring[((size_t) b * p.ring + ((p.pos[b] + t) & (p.ring - 1))) * Cc + col];
         }
-        for (int t = 0; t < C; t += 8) {
-            float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = t + i < n ? x[(size_t) (t + i) * Cc] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float y = w.x * h[0];
-                y = fmaf(w.y, h[1], y);
-                y = fmaf(w.z, h[2], y);
-                y = fmaf(w.w, v[i], y);
-                rows[part][(t + i) * RS + ch] = t + i < n ? silu_(y) : 0.0f;
-                h[0] = h[1];
-                h[1] = h[2];
-                h[2] = v[i];
-            }
+        for (int t = 0; t < C; ++t) {
+            float y = w.x * h[0];
+            y = fmaf(w.y, h[1], y);
+            y = fmaf(w.z, h[2], y);
+            y = fmaf(w.w, v[t], y);
+            rows[part][t * RS + ch] = t < n ? silu_(y) : 0.0f;
+            h[0] = h[1];
+            h[1] = h[2];
+            h[2] = v[t];
         }
     } else {
-        for (int i = tid; i < 2 * C * (D / 4); i += 256) {
-            const int part = i >> 11, t = (i >> 5) & (C - 1), d = (i & 31) * 4;
-            const float *src = (part ? p.k : p.q) + ((row0 + t) * p.nkh + kh) * D + d;
-            *reinterpret_cast<float4 *>(&rows[part][t * RS + d]) = t < n ? *reinterpret_cast<const float4 *>(src) : f4(0.0f);
+        float4 x[16];  // all requested before the first is waited for
+        const uint32_t pitch = p.nkh * D * 4, at = (tid >> 5) * pitch + (tid & 31) * 16;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const brsrc rd = buf((i < 8 ? p.q : p.k) + (row0 * p.nkh + kh) * D, (uint32_t) (n - 1) * pitch + D * 4);  // rows behind: 0
+            x[i] = bld4(rd, at + i % 8 * 8 * pitch, 0);
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            *reinterpret_cast<float4 *>(&rows[i / 8][((tid >> 5) + i % 8 * 8) * RS + (tid & 31) * 4]) = x[i];
     }
-    __syncthreads();
+    lds_barrier();
     {  // the row's norm and largest value, by two threads
         const int part = tid >> 7, t = (tid >> 1) & (C - 1);
         const float *x = &rows[part][t * RS + (tid & 1) * (D / 2)];
@@ -155,9 +170,9 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
             back[part][t] = pow2(e);
         }
     }
-    __syncthreads();
+    lds_barrier();
     // 2. operands.  Row operand (q, k): lane = row 16 wave + l%16, slot j of step s = dim 32 s + 16 (j / 4) + 4 (l / 16) + j % 4
-    v4u qh[4], ql[4], kh_[4], kl[4], kt[2][2][2];
+    v4u qh[4], ql[4], kh_[4], kl[4];
     {
         const int t = 16 * wave + r;
 #pragma unroll
@@ -188,20 +203,21 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                     const int u = 32 * s + 16 * (j / 4) + 4 * q4 + j % 4;
                     v[j] = rows[1][u * RS + 32 * wave + 16 * c + r] * mul[1][u];
                 }
-                split8(v, kt[c][s][0], kt[c][s][1]);
+                v4u hi, lo;
+                split8(v, hi, lo);
                 uint8_t *d = kd + KT + (((wave * 2 + c) * 2 + s) * 2) * FRAG + lane * 16;
-                *reinterpret_cast<v4u *>(d) = kt[c][s][0];
-                *reinterpret_cast<v4u *>(d + FRAG) = kt[c][s][1];
+                *reinterpret_cast<v4u *>(d) = hi;
+                *reinterpret_cast<v4u *>(d + FRAG) = lo;
             }
     }
-    __syncthreads();
+    lds_barrier();
     v4u *op = reinterpret_cast<v4u *>(rows[0]);  // [tile][step][hi, lo][lane]: K's row operands, later two forms of M
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         op[((wave * 4 + s) * 2) * 64 + lane] = kh_[s];
         op[((wave * 4 + s) * 2 + 1) * 64 + lane] = kl[s];
     }
-    __syncthreads();
+    lds_barrier();
     // 3. k_j.k_i and k_j.q_i of the wave's 16 rows i (lane: i = 16 wave + l%16, j = 16 tile + 4 (l / 16) + e)
     v4f kk[4], qk[4];
 #pragma unroll
@@ -230,23 +246,22 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
     }
     // 4. each value head of the key head
     float *A = rows[1], *Md = rows[1] + C * AS;
-    const int per = p.nvh / p.nkh, Cc = 2 * p.nkh * D + p.nvh * D;
     for (int hi_ = 0; hi_ < per; ++hi_) {
-        const int h = p.head_map == 0 ? kh + hi_ * p.nkh : kh * per + hi_;
+        asm volatile("" : "+v"(r), "+v"(q4));  // addresses are made again for each head, not kept in some 60 registers
+        const int h = head_of(hi_);
         uint8_t *hd = a.heads + ((size_t) item * p.nvh + h) * HEAD_BYTES;
         float *gd = reinterpret_cast<float *>(hd + GATES);
         float be = 0.0f, g = 0.0f;
         if (lane < n) {
-            const size_t t = row0 + lane;
+            be = gate[0];
+            g = gate[1];
             if (BLOCK) {
-                const float ga = p.ab[t * 2 * p.nvh + h] + p.dt_bias[h];
-                be = sigmoidf_(p.ab[t * 2 * p.nvh + p.nvh + h]);
+                const float ga = g + p.dt_bias[h];
+                be = sigmoidf_(be);
                 g = (ga > 20.0f ? ga : log1pf(expf(ga))) * p.ssm_a[h];
-            } else {
-                be = p.beta[t * p.nvh + h];
-                g = p.g[t * p.nvh + h];
             }
         }
+        if (hi_ + 1 < per) request_gates(hi_ + 1);
         double gs = fmax((double) g, -200.0);  // a decay below e^-200 is 0 in fp32 (and -infinity would cancel to NaN)
         if (g != g) gs = g;
 #pragma unroll
@@ -254,7 +269,7 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
             const double y = __shfl_up(gs, d);
             if (lane >= d) gs += y;
         }
-        __syncthreads();  // what the last head left in the LDS has been read
+        lds_barrier();  // what the last head left in the LDS has been read
         if (wave == 0) {
             const double g63 = __shfl(gs, 63);
             const float eg = expf((float) gs), up = expf((float) (g63 - gs)) * back[1][lane], um = wave_max(up);
@@ -268,7 +283,31 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                 gd[G_SC + 2] = expf((float) g63);
             }
         }
-        __syncthreads();
+        lds_barrier();
+        // values of the wave's columns 32 wave + 16 c + l%16, requested ahead
+        float vv[2][2][8], before[2][3];
+        float4 cw[2];
+        {
+            const int pitch = BLOCK ? Cc : p.nvh * D, col = (BLOCK ? 2 * p.nkh * D : 0) + h * D + 32 * wave + r;
+            const brsrc v = buf((BLOCK ? p.qkv : p.v) + row0 * pitch, (uint32_t) n * pitch * 4);  // rows behind: 0
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if (BLOCK) {
+                    const int ch = col + 16 * c;
+                    cw[c] = *reinterpret_cast<const float4 *>(p.conv_w + 4 * ch);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        before[c][i] = t0 ? p.qkv[(row0 + i - 3) * Cc + ch]
+                                          : p.conv_ring[((size_t) b * p.ring + ((p.pos[b] + i - 3) & (p.ring - 1))) * Cc + ch];
+                }
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        vv[c][s][j] = bld(v, (uint32_t) ((32 * s + 16 * (j / 4) + 4 * q4 + j % 4) * pitch + col + 16 * c) * 4, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         const double gi = G[16 * wave + r];
         const float bi = bet[16 * wave + r];
         {
@@ -304,51 +343,35 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                     *reinterpret_cast<v4u *>(d + FRAG) = lo;
                 }
         }
-        // values of the wave's columns 32 wave + 16 c + l%16 (slots as in k^T), requested ahead
-        float vv[2][2][8];
+        // values of the wave's columns 32 wave + 16 c + l%16 (slots as in k^T)
         if (BLOCK) {
-            const int ch0 = 2 * p.nkh * D + h * D + 32 * wave + r;
-            // rows behind the last, and before a request's first, read as 0; the latter are then taken from the ring
-            const brsrc xb = buf(p.qkv + (row0 - (t0 ? 3 : 0)) * Cc, (uint32_t) (n + (t0 ? 3 : 0)) * Cc * 4);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int ch = ch0 + 16 * c;
-                const float4 w = *reinterpret_cast<const float4 *>(p.conv_w + 4 * ch);
+                float y[3] = {before[c][0], before[c][1], before[c][2]};  // the three tokens before four of the lane's
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {  // four tokens in a row
-                    const int u0 = 16 * g + 4 * q4;
-                    float y[7];
+                for (int g = 0; g < 4; ++g) {
+                    float *x = &vv[c][g / 2][4 * (g % 2)], nx[3];
 #pragma unroll
-                    for (int i = 0; i < 7; ++i) y[i] = bld(xb, (uint32_t) (((u0 + i - (t0 ? 0 : 3)) * Cc + ch) * 4), 0);
-                    if (g == 0 && t0 == 0 && q4 == 0) {
-#pragma unroll
-                        for (int i = 0; i < 3; ++i)
-                            y[i] = p.conv_ring[((size_t) b * p.ring + ((p.pos[b] + i - 3) & (p.ring - 1))) * Cc + ch];
+                    for (int i = 0; i < 3; ++i) {  // a quarter's last three are the next quarter's, the last quarter's the next g's
+                        const float z = __shfl(x[i + 1], (lane + 48) & 63);
+                        if (q4) y[i] = z;
+                        nx[i] = z;
                     }
+                    const float in[7] = {y[0], y[1], y[2], x[0], x[1], x[2], x[3]};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float z = w.x * y[i];
-                        z = fmaf(w.y, y[i + 1], z);
-                        z = fmaf(w.z, y[i + 2], z);
-                        z = fmaf(w.w, y[i + 3], z);
-                        vv[c][g / 2][4 * (g % 2) + i] = u0 + i < n ? silu_(z) : 0.0f;
+                        float z = cw[c].x * in[i];
+                        z = fmaf(cw[c].y, in[i + 1], z);
+                        z = fmaf(cw[c].z, in[i + 2], z);
+                        z = fmaf(cw[c].w, in[i + 3], z);
+                        x[i] = 16 * g + 4 * q4 + i < n ? silu_(z) : 0.0f;
                     }
-                    if (g % 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) y[i] = nx[i];
                 }
             }
-        } else {
-            const brsrc v = buf(p.v + row0 * p.nvh * D + h * D, (uint32_t) ((n - 1) * p.nvh * D + D) * 4);  // rows behind: 0
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int u = 32 * s + 16 * (j / 4) + 4 * q4 + j % 4;
-                        vv[c][s][j] = bld(v, (uint32_t) (u * p.nvh * D + 32 * wave + 16 * c + r) * 4, 0);
-                    }
         }
-        __syncthreads();
+        lds_barrier();
         {  // the inverse of the wave's diagonal block, lane = column l%16, by substitution
             float x[16];
 #pragma unroll
@@ -364,7 +387,7 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                 for (int i = 0; i < 16; ++i) Md[(16 * wave + i) * MS + r] = x[i];
             }
         }
-        __syncthreads();
+        lds_barrier();
         // the wave's block row of M, from the diagonal leftwards: M_wj = -(sum_(k > j) M_wk A_kj) M_jj, as transposes, whose
         // products leave a lane with row l%16 and columns 4 (l / 16) + e: the layout they are needed in next
         v4f mt[4];
@@ -393,6 +416,10 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                 o = __builtin_amdgcn_mfma_f32_16x16x4f32(Md[(16 * j + 4 * q4 + e) * MS + r], t[e], o, 0, 0, 0);
             mt[j] = -o;
         }
+        // K^T of the wave's dims comes back from where the lane has put it (32 registers less through the rest of the loop)
+        v4u kt[2][2][2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kt[i / 4][i / 2 % 2][i % 2] = *reinterpret_cast<v4u *>(kd + KT + (wave * 8 + i) * FRAG + lane * 16);
         // M diag(beta e^G 2^ek) and M diag(beta) as operands, a scale a row
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
@@ -421,7 +448,7 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                     split8(x, d[0], d[64]);
                 }
         }
-        __syncthreads();
+        lds_barrier();
         const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
         // U0 of the wave's columns: lane = column, tokens 16 i + 4 (l / 16) + e
 #pragma unroll
@@ -495,7 +522,7 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                 wsq[wave][16 * i + r] = sq;
             }
         }
-        __syncthreads();
+        lds_barrier();
         // W as the scan's row operand: step `wave` of every row tile
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
