@@ -877,7 +877,7 @@ int kv4_pick_nsplit(int B, int T, int nq, int nkv, int ctx) {
     // A split costs a row of sums that is written and read again, so the time is about u keys / nsplit + w nsplit, least at
     // a multiple of sqrt(keys).  One token, 2 kv heads, us at 16, 32, 64, 128, 256 splits: 4k keys 25.0, 24.1, 24.7, 27.0,
     // 32.6; 32k keys 43.4, 34.4, 30.6, 32.2, 38.9; 100k keys 86.5, 58.4, 45.4, 45.0, 52.1.
-    const int most = std::max(1, (int) (std::sqrt((double) ctx) * 0.5));
+    const int most = std::max(1, (int) (std::sqrt((double) std::max(ctx, 1)) * 0.5));
     return (int) std::min<long long>(want, most);
 }
 

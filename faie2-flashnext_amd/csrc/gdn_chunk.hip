@@ -861,6 +861,7 @@ int gdn_chunk_launch(const GdnChunk &p, hipStream_t st) {
     if (p.nvh % p.nkh) FN_FAIL("gdn_chunk: nvh must be a multiple of nkh");
     if (p.head_map != 0 && p.head_map != 1) FN_FAIL("gdn_chunk: head_map must be 0 (tiled h % nkh) or 1 (grouped)");
     if (p.B > 65535 || p.nkh > 65535) FN_FAIL("gdn_chunk: B and nkh must be <= 65535");
+    if (p.nvh > 32768) FN_FAIL("gdn_chunk: nvh must be <= 32768 (the offsets in a chunk are 32-bit)");
     if (!p.cu || !p.S || !p.o || !p.work) FN_FAIL("gdn_chunk: null pointer");
     if (block) {
         if (p.gate_act != 0 && p.gate_act != 1) FN_FAIL("gdn_chunk: gate_act must be 0 (sigmoid) or 1 (silu)");

@@ -282,7 +282,9 @@ int fn_test_attn_qsa(int B, int nq, int nkv, int hd, int nrot, float theta, floa
  *     lengths in one call.  Request b's new tokens are rows cu[b] .. cu[b + 1] - 1 of every per-token array of T rows; rows
  *     from cu[B] on are left as they were.  past [B] are the tokens that each request already has (0 for a new one).
  *     Nothing is allocated and no memset is recorded; a call can be captured into a graph and replayed with new
- *     contents of its buffers.  What the device finds wrong is recorded in the status word (fn_dev_status).
+ *     contents of its buffers.  A workspace holds nothing between calls; calls that may run at the same time (two streams,
+ *     two graphs) need one each.  All buffers are on the device that is current at the call.  cu does not decrease.  What
+ *     the device finds wrong is recorded in the status word (fn_dev_status).
  * ====================================================================================================== */
 
 /* Page tables.  The cache is npages pages of 64 tokens; table [B][max_blocks] names the page of each 64-token block of
@@ -322,7 +324,9 @@ int fn_kv4_unpack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, c
  * the request's keys up to its own position as the cache holds them (a block whose table entry is outside the cache is
  * passed over; a query that finds no key gets zeros).  The rotation's angle is taken in 64 bits.  nq / nkv any whole number.
  * nsplit: key splits of a row (fn_attn_kv4_nsplit: the choice for contexts of up to ctx keys).  All arrays but the
- * int32 ones 16-byte aligned; work: fn_attn_kv4_work_bytes() bytes. */
+ * int32 ones 16-byte aligned; work: fn_attn_kv4_work_bytes() bytes.  The slots of one call (other than -1) are different.
+ * Requests may name the same pages in their tables.  A row whose seq is not the request whose rows it lies in is not
+ * cached, its output is undefined, and the status word says so. */
 int fn_attn_kv4_dev(int B, int T, int nq, int nkv, int hd, int nrot, float theta, float eps, int max_blocks, int npages,
                     const int32_t *past, const int32_t *cu, const int32_t *table, const int32_t *slot,
                     const int32_t *seq, const float *qg, const float *k, const float *v, const float *wq,
@@ -334,7 +338,7 @@ int fn_attn_kv4_nsplit(int B, int T, int nq, int nkv, int ctx);
  * v [T][nvh][dv], beta, g [T][nvh], cu [B + 1], S [B][nvh][dk][dv] in/out, o [T][nvh][dv].  The state of a request without
  * new tokens is left as it was.  An infinity or NaN in a request's inputs may reach all outputs of its value head from
  * the start of the 64 tokens that hold it.  q, k, o and work 16-byte aligned; work: fn_gdn_chunk_work_bytes(B, T, nkh, nvh)
- * bytes.  For one or a few tokens a request fn_gdn_core_dev and fn_gdn_block_dev are the faster calls. */
+ * bytes.  nvh up to 32768.  For one or a few tokens a request fn_gdn_core_dev and fn_gdn_block_dev are the faster calls. */
 int fn_gdn_core_chunk_dev(int B, int T, int nkh, int nvh, int dk, int dv, int head_map, const int32_t *cu, const float *q,
                           const float *k, const float *v, const float *beta, const float *g, float *S, float *o,
                           void *work, size_t work_bytes, void *stream);
