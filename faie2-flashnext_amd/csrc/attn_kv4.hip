@@ -542,6 +542,31 @@ __global__ void __launch_bounds__(WAVES * 64, 3) k_attn_kv4(const Kv4Args a) {
     }
 }
 
+// The item of workgroup z, and its request (-1: none): the requests with the most keys first, each from its last rows on.
+// The workgroups of a call last as long as their keys; in the order of the items the last round of a mixed batch is begun
+// late by its longest (24 requests of 1 or 300 tokens over 0.8k to 8k keys: 689 us, in this order 573 us).  A wave ranks up
+// to 64 requests, one a lane; beyond that a call has many rounds, and the order is that of the items.
+__device__ __forceinline__ int longest_first(const Kv4Args &a, int rt, int z, int &item) {
+    const int lane = threadIdx.x & 63;
+    if (a.B > 64) {
+        item = a.items - 1 - z;
+        return request_of(a.cu, a.B, item, a.grp, rt);
+    }
+    const int lb = min(lane, a.B - 1), c0 = a.cu[lb], n = max(0, min(a.cu[lb + 1], a.T) - c0), past = a.past[lb];
+    const int keys = past < 0 ? 0 : min(past, a.mb * PG) + n;
+    const int cnt = lane < a.B && c0 >= 0 ? (n * a.grp + rt - 1) / rt : 0;
+    int before = 0;
+    for (int i = 0; i < a.B; ++i) {
+        const int k = __builtin_amdgcn_readlane(keys, i), c = __builtin_amdgcn_readlane(cnt, i);
+        before += k > keys || (k == keys && i < lane) ? c : 0;
+    }
+    const uint64_t hit = __ballot(z >= before && z < before + cnt);
+    if (!hit) return -1;
+    const int b = __ffsll((unsigned long long) hit) - 1;
+    item = first_item(a.cu, b, a.grp, rt) + __builtin_amdgcn_readlane(cnt, b) - 1 - (z - __builtin_amdgcn_readlane(before, b));
+    return b;
+}
+
 // grid (nsplit, nkv, items), four waves: the 32 rows of an item against the keys of a split, 128 keys at a time.  For the
 // scores a wave takes 32 of the keys, for the values a quarter of the dims: so each value is converted once for all rows,
 // the sums of a wave are 32 registers and not 128 (which left one wave a SIMD: 463 us for what now takes 340), and nothing
@@ -549,15 +574,17 @@ __global__ void __launch_bounds__(WAVES * 64, 3) k_attn_kv4(const Kv4Args a) {
 // the probabilities.
 // What bounds it: 136 matrix instructions of 16 cycles and some 600 vector instructions of 4 a wave and step, which two
 // waves a SIMD overlap in part, and 240 KB a step through the LDS.  A prompt of 4001 tokens, 16 + 2 heads: 340 us, the
-// matrix instructions alone 113 us; 24 requests of 1 to 300 tokens over up to 8k keys: 683 us, 329 us.
+// matrix instructions alone 113 us; 24 requests of 1 or 300 tokens over 0.8k to 8k keys: 573 us, 197 us.
 __global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a) {
     constexpr int RT = 16 * NRB, STEP = WAVES * 32;
     __shared__ __align__(16) uint8_t lq[NRB * QBLK];
     __shared__ v4u lp[WAVES][NRB][3][64];  // probabilities of 32 keys: [row block][part]
     __shared__ float lm[WAVES][RT], ll[WAVES][RT];
-    const int sp = blockIdx.x, g = blockIdx.y, item = a.items - 1 - (int) blockIdx.z;  // the longest rows first
+    const int sp = blockIdx.x, g = blockIdx.y;
+    int item;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15;
-    const int b = request_of(a.cu, a.B, item, a.grp, RT);
+    const int b = longest_first(a, RT, blockIdx.z, item);
+    if (b < 0 || item < 0 || item >= a.items) return;
     const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r0 = (item - first_item(a.cu, b, a.grp, RT)) * RT;
     const int rows = n * a.grp;
     if (c0 < 0 || r0 < 0 || r0 >= rows) return;
