@@ -91,14 +91,10 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
     __shared__ double krow[PART == PREP_QUERIES ? 1 : WAVES][MAXROT];
     __shared__ float qrow[PART == PREP_KEYS ? 1 : WAVES][8][MAXROT + 4];
     const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int total = min(a.cu[a.B], a.T);
-    if (t >= total) return;
-    const int b = a.seq[t];
-    if (b < 0 || b >= a.B || t < a.cu[b] || t >= a.cu[b + 1] || a.cu[b] < 0) {
-        if (threadIdx.x == 0) atomicOr(a.status, FN_STATUS_ROWS);
-        return;
-    }
-    // the wave's first rows are requested before anything that waits
+    // the wave's first rows, and what else depends on no other load, are requested before anything that waits
+    const int slot = a.slot[t], half = a.nrot / 2;
+    auto freq = [&](int d) { return a.freq[d < half ? d : d < a.nrot ? d - half : 0]; };
+    double fr = freq(threadIdx.x);
     const int waves = blockDim.x >> 6, octets = (a.nq + 7) / 8;
     const int from = PART == PREP_QUERIES ? 2 * a.nkv : 0, tasks = 2 * a.nkv + (PART == PREP_KEYS ? 0 : octets);
     const int first = from + wave + waves * blockIdx.y;
@@ -114,19 +110,25 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
         }
     };
     if (first < tasks) request(first);
+    const int total = min(a.cu[a.B], a.T);
+    if (t >= total) return;
+    const int b = a.seq[t];
+    if (b < 0 || b >= a.B || t < a.cu[b] || t >= a.cu[b + 1] || a.cu[b] < 0) {
+        if (threadIdx.x == 0) atomicOr(a.status, FN_STATUS_ROWS);
+        return;
+    }
     const long long P = (long long) a.past[b] + (t - a.cu[b]);
     if ((a.past[b] < 0 || P >= (long long) a.mb * PG) && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_POS);
-    const int half = a.nrot / 2;
     // the angle in 64 bits: a float product is off by up to half a radian at a million tokens
     for (int d = threadIdx.x; d < MAXROT; d += blockDim.x) {
         double sv = 0.0, cv = 1.0;
-        if (d < a.nrot) sin_cos((double) P * a.freq[d < half ? d : d - half], sv, cv);
+        if (d != threadIdx.x) fr = freq(d);
+        if (d < a.nrot) sin_cos((double) P * fr, sv, cv);
         if (d < half) sv = -sv;
         cs[d] = cv, sn[d] = sv;
         cf[d] = (float) cv, sf[d] = (float) sv;
     }
     __syncthreads();
-    const int slot = a.slot[t];
     const bool put = slot >= 0 && slot / PG < a.npages;
     if (PART != PREP_QUERIES && slot >= 0 && !put && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_PAGE);
     for (int task = first; task < tasks; task += waves * gridDim.y) {
@@ -832,24 +834,44 @@ template <int RT>
 __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
     __shared__ float4 part[WAVES][HD / 4];
     __shared__ float pl[WAVES];
-    const int item = blockIdx.x / RT, g = blockIdx.y, row = blockIdx.x % RT, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int item = blockIdx.x / RT, g = blockIdx.y, row = blockIdx.x % RT, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = request_of(a.cu, a.B, item, a.grp, RT);
     const int c0 = a.cu[b], n = min(a.cu[b + 1], a.T) - c0, r = (item - first_item(a.cu, b, a.grp, RT)) * RT + row;
     if (c0 < 0 || r < 0 || r >= n * a.grp) return;
+    // the gate and the sums of the wave's first splits are requested before the references are there
+    const int t = r / a.grp;
+    const size_t at = (size_t) (c0 + t) * a.nq + g * a.grp + (r - t * a.grp);
+    const float4 z = reinterpret_cast<const float4 *>(a.qg + (at * 2 + 1) * HD)[lane];
     const size_t at0 = ((size_t) item * a.nkv + g) * a.nsplit * RT + row;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml);
+    constexpr int AHEAD = 8;
+    float4 po[AHEAD];
+    float2 pm[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        if (wave + i * WAVES >= a.nsplit) break;
+        const size_t p = at0 + (size_t) (wave + i * WAVES) * RT;
+        pm[i] = ml[p];
+        po[i] = reinterpret_cast<const float4 *>(a.part_o + p * HD)[lane];
+    }
     float M = -INFINITY;
     for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, ml[at0 + (size_t) s * RT].x);
     M = wave_max(M);
     float L = 0.0f;
     float4 o = f4(0.0f);
-#pragma unroll 4
-    for (int s = wave; s < a.nsplit; s += WAVES) {
-        const size_t at = at0 + (size_t) s * RT;
-        const float2 x = ml[at];
+    auto join = [&](const float2 &x, const float4 &y) {
         const float f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x.x - M) * SM_SCALE);
         L = fmaf(x.y, f, L);
-        o = add_scaled(o, reinterpret_cast<const float4 *>(a.part_o + at * HD)[lane], f);
+        o = add_scaled(o, y, f);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (wave + i * WAVES < a.nsplit) join(pm[i], po[i]);
+#pragma unroll 4
+    for (int s = wave + AHEAD * WAVES; s < a.nsplit; s += WAVES) {
+        const size_t p = at0 + (size_t) s * RT;
+        join(ml[p], reinterpret_cast<const float4 *>(a.part_o + p * HD)[lane]);
     }
     part[wave][lane] = o;
     if (lane == 0) pl[wave] = L;
@@ -860,9 +882,6 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
         o = add_scaled(o, part[w][lane], 1.0f);
         L += pl[w];
     }
-    const int t = r / a.grp;
-    const size_t at = (size_t) (c0 + t) * a.nq + g * a.grp + (r - t * a.grp);
-    const float4 z = reinterpret_cast<const float4 *>(a.qg + (at * 2 + 1) * HD)[lane];
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     reinterpret_cast<float4 *>(a.og + at * HD)[lane] = make_float4(
         o.x * inv * sigmoidf_(z.x), o.y * inv * sigmoidf_(z.y), o.z * inv * sigmoidf_(z.z), o.w * inv * sigmoidf_(z.w));
