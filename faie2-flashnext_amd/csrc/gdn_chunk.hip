@@ -12,7 +12,7 @@
 //   k_chunk_scan, one a (request, value head, columns of S), which walks the request's chunks with its columns of S in
 //     registers: three small products one after the other a chunk, and two exchanges through the LDS.
 // W and U0 are formed before the scan, not M inside it: the scan is the sequential part, and M there is one more product
-// and exchange a chunk (15k tokens, 32 value heads: scan 596 us with M, 405 us with W; the other kernel 252 and 278 us).
+// and exchange a chunk (15k tokens, 32 value heads: scan 596 us with M, 405 us with W; the other kernel 252 and 272 us).
 // Products: an fp32 operand is two f16 values (hi and lo, 11 bits each) under a power-of-two scale, and a product is hi
 // hi + hi lo + lo hi on v_mfma_f32_16x16x32_f16: what is left out is 2^-22 of a product at the worst and 2^-24 in the
 // mean, in half the instructions of six bf16 products and a fifth of the time of fp32 ones.  f16's range is met by
@@ -77,14 +77,22 @@ __device__ __forceinline__ void split8(const float (&x)[8], v4u &hi, v4u &lo) {
 __device__ __forceinline__ int exp_of(float x) { return x > 0.0f ? max(-100, min(126, (int) (__float_as_uint(x) >> 23) - 127)) : 0; }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t) (e + 127) << 23); }
 
-__device__ __forceinline__ float silu_(float x) { return x * __builtin_amdgcn_rcpf(1.0f + expf(-x)); }
+// e^x = 2^t (1 + r log 2), t = x log2 e as rounded and r what the rounding left, with log2 e in two parts: off by less than
+// 2^-22 of the value.  0 below fp32's normal range; beyond it no finite value.
+__device__ __forceinline__ float exp_(float x) {
+    const float t = x * 1.44269504f, r = fmaf(x, 1.925963e-8f, fmaf(x, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * 0.693147181f, e);
+}
+// (bounded so that e^-x is finite: what x would make of it beyond is below 2^-120)
+__device__ __forceinline__ float silu_(float x) { return x * __builtin_amdgcn_rcpf(1.0f + exp_(fminf(-x, 88.0f))); }
 
 __device__ __forceinline__ float4 lds4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 
 // grid (chunks, nkh), four waves.  What bounds it: memory.  15k tokens, 16 key and 32 value heads: 0.49 GB of q, k, v in,
-// 0.86 GB of operands out in 278 us, 4.9 TB/s (all rows are requested before the first is waited for, and V and the gates
-// a part ahead: 332 us without).  In the block form, 4k tokens, 16 and 48 heads: 0.49 GB in 149 us, 3.2 TB/s; it uses all
-// 256 registers, and a chunk's three value heads one after the other leave two rounds of workgroups.  M = (I + A)^-1 by blocks of 16: a wave inverts its diagonal block by
+// 0.86 GB of operands out in 272 us, 5.0 TB/s (all rows are requested before the first is waited for, and V and the gates
+// a part ahead: 332 us without).  In the block form, 4k tokens, 16 and 48 heads: 0.49 GB in 139 us, 3.5 TB/s: half of its
+// time goes to vector instructions (conv and SiLU of every channel), and a chunk's three value heads one after the other
+// leave two rounds of workgroups.  M = (I + A)^-1 by blocks of 16: a wave inverts its diagonal block by
 // substitution, one column a lane, and forms its block row from the diagonal leftwards on fp32 matrix instructions.
 template <bool BLOCK>
 __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
@@ -318,7 +326,7 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int jt = 16 * j + 4 * q4 + e, it = 16 * wave + r;
-                    const float dec = j <= wave && jt <= it ? expf((float) (gi - G[jt])) : 0.0f;
+                    const float dec = j <= wave && jt <= it ? exp_((float) (gi - G[jt])) : 0.0f;
                     av[e] = j <= wave && jt < it ? bi * dec * kk[j][e] : 0.0f;
                     pv[j][e] = j <= wave && jt <= it ? dec * qk[j][e] : 0.0f;
                     pm = fmaxf(pm, fabsf(pv[j][e]));
