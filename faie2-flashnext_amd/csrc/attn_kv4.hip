@@ -279,7 +279,7 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), bf16x2));
 }
 constexpr float SM_SCALE = 0.0625f * 1.4426950408889634f;  // 1 / sqrt(HD), and the softmax in powers of two
-constexpr float SLACK = 8.0f * 16.0f;                      // growth of a row's largest raw score that moves its reference
+constexpr float SLACK = 8.0f;                              // growth of a row's largest score, in powers of two, that moves its reference
 constexpr float PUP = 16.0f;                               // probabilities times 2^16: the parts of the least ones stay normal
 
 // 64 dims of the lane's eight keys as bf16 pairs: dims 32 t + 2 (l % 16), + 1
@@ -320,7 +320,9 @@ struct KvBlock {
     __device__ __forceinline__ void values(int t, uint32_t (&x)[8]) const { values_of(v[t / 2], vs[t / 2], t % 2, x); }
 };
 
-// The state of one row (the lane's column) of an online softmax.  MASK: keys from lim on count for nothing.
+// The state of one row (the lane's column) of an online softmax.  The reference m is a whole power of two near the row's
+// largest: a probability is then one fused multiply-add and one exponential away from its score, and every factor between
+// references (of keys before, of other waves and splits) is a power of two, exact.  MASK: keys from lim on count for nothing.
 struct Softmax {
     float m = -INFINITY, l = 0.0f;
     // eight raw scores (key + 16 (i / 4) + i % 4), those behind the mask -infinity; returns the largest of the lane's row
@@ -335,13 +337,14 @@ struct Softmax {
     }
     // -> probabilities 2^PUP p; returns the factor of what was summed before
     template <bool MASK> __device__ __forceinline__ float step(const float (&s)[8], float mx, float (&p)[8]) {
-        const bool first = m == -INFINITY, moved = !first && mx > m + SLACK;
-        const float mn = first || moved ? mx : m;
-        const float corr = moved ? __builtin_amdgcn_exp2f((m - mn) * SM_SCALE) : 1.0f;
+        const float top = rintf(mx * SM_SCALE);
+        const bool first = m == -INFINITY, moved = !first && top > m + SLACK;
+        const float mn = first || moved ? top : m, up = PUP - mn;
+        const float corr = moved ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
         float ps = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i] - mn, SM_SCALE, PUP));
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], SM_SCALE, up));
             if (MASK && s[i] == -INFINITY) p[i] = 0.0f;
             ps += p[i];
         }
@@ -420,26 +423,25 @@ __global__ void __launch_bounds__(WAVES * 64, 3) k_attn_kv4(const Kv4Args a) {
         next = page_of(kb + 2 * WAVES);
         const bool in = ok(here);  // a block outside the cache counts for nothing
         if (!in && lane == 0) atomicOr(a.status, FN_STATUS_PAGE);
-        // scores, in two sums: what the first part of the queries gives, and the small rest
+        // scores, the small parts of the queries first
         float S[8];
-        v4f big[2] = {zero, zero}, small[2] = {zero, zero};
+        v4f acc[2] = {zero, zero};
 #define FN_KV4_SLOT(U, P)                                                                              \
     do {                                                                                              \
         const v6u q = operand(((U) * HSLOT + (P)) * FRAG);                                             \
-        v4f(&acc)[2] = (P) == 0 ? big : small;                                                         \
         acc[0] = mma_k<(U), (P)>(x.k[0][U], (int) x.ks, q, (int) hs[U], acc[0]);                       \
         acc[1] = mma_k<2 + (U), (P)>(x.k[1][U], (int) x.ks, q, (int) hs[U], acc[1]);                   \
     } while (0)
-        FN_KV4_SLOT(0, 1);
-        FN_KV4_SLOT(0, 0);
         FN_KV4_SLOT(0, 2);
-        FN_KV4_SLOT(1, 0);
-        FN_KV4_SLOT(1, 1);
         FN_KV4_SLOT(1, 2);
+        FN_KV4_SLOT(0, 1);
+        FN_KV4_SLOT(1, 1);
+        FN_KV4_SLOT(0, 0);
+        FN_KV4_SLOT(1, 0);
 #undef FN_KV4_SLOT
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float s = big[i / 4][i % 4] + small[i / 4][i % 4];
+            const float s = acc[i / 4][i % 4];
             S[i] = s + dpp_ror<8>(s);
         }
         x.load_k(p, kn & 1, lane);
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(WAVES * 64, 3) k_attn_kv4(const Kv4Args a) {
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
             const float mw = wm[w][row];
-            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - M) * SM_SCALE);
+            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
             L = fmaf(wl[w][row], f, L);
             s = add_scaled(s, *reinterpret_cast<const float4 *>(mo + (w * RT + row) * MS + d), f);
         }
@@ -531,8 +533,8 @@ __global__ void __launch_bounds__(WAVES * 64, 3) k_attn_kv4(const Kv4Args a) {
             const float4 z = *reinterpret_cast<const float4 *>(a.qg + (at * 2 + 1) * HD + d);
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees no key: zeros
             *reinterpret_cast<float4 *>(a.og + at * HD + d) =
-                make_float4(s.x * inv * sigmoidf_(z.x), s.y * inv * sigmoidf_(z.y), s.z * inv * sigmoidf_(z.z),
-                            s.w * inv * sigmoidf_(z.w));
+                make_float4(s.x * inv * gate_of(z.x), s.y * inv * gate_of(z.y), s.z * inv * gate_of(z.z),
+                            s.w * inv * gate_of(z.w));
         } else {
             const size_t at = (((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + row;
             *reinterpret_cast<float4 *>(a.part_o + at * HD + d) = s;
@@ -658,38 +660,37 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a
         const int own = wave < 2 ? page[0] : page[1];
         const bool in = kb < k1 && ok(own);  // a block outside the cache counts for nothing
         if (kb < k1 && !in && lane == 0) atomicOr(a.status, FN_STATUS_PAGE);
-        // scores, in two sums: what the first part of the queries gives, and the small rest
+        // scores, the small parts of the queries first
         float S[NRB][8];
         {
-            v4f big[2][NRB], small[2][NRB];
+            v4f acc[2][NRB];
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
-                for (int j = 0; j < NRB; ++j) big[hb][j] = small[hb][j] = zero;
+                for (int j = 0; j < NRB; ++j) acc[hb][j] = zero;
 #define FN_KV4_PART(U, P)                                                                                            \
     do {                                                                                                            \
         _Pragma("unroll") for (int j = 0; j < NRB; ++j) {                                                            \
             const v6u q = operand(j * QBLK + ((U) * NPART + (P)) * FRAG);                                            \
-            v4f(&acc)[2][NRB] = (P) == 0 ? big : small;                                                              \
             acc[0][j] = mma_k<(U), (P) % 4>(k[0][U], (int) ks, q, (int) qs[j][U][(P) / 4], acc[0][j]);               \
             acc[1][j] = mma_k<2 + (U), (P) % 4>(k[1][U], (int) ks, q, (int) qs[j][U][(P) / 4], acc[1][j]);           \
         }                                                                                                           \
     } while (0)
-            FN_KV4_PART(0, 0);
-            FN_KV4_PART(0, 1);
-            FN_KV4_PART(0, 2);
-            FN_KV4_PART(0, 3);
             FN_KV4_PART(0, 4);
-            FN_KV4_PART(1, 0);
-            FN_KV4_PART(1, 1);
-            FN_KV4_PART(1, 2);
-            FN_KV4_PART(1, 3);
             FN_KV4_PART(1, 4);
+            FN_KV4_PART(0, 3);
+            FN_KV4_PART(1, 3);
+            FN_KV4_PART(0, 2);
+            FN_KV4_PART(1, 2);
+            FN_KV4_PART(0, 1);
+            FN_KV4_PART(1, 1);
+            FN_KV4_PART(0, 0);
+            FN_KV4_PART(1, 0);
 #undef FN_KV4_PART
 #pragma unroll
             for (int j = 0; j < NRB; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) S[j][i] = big[i / 4][j][i % 4] + small[i / 4][j][i % 4];
+                for (int i = 0; i < 8; ++i) S[j][i] = acc[i / 4][j][i % 4];
         }
         __builtin_amdgcn_sched_barrier(0);
         load_k(next);
@@ -731,22 +732,20 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a
 #pragma unroll
                 for (int t = 0; t < 4; ++t) o[j][t / 2][t % 2] *= corr[j];
         }
+        if (at + STEP > k1 || !ok(page[0]) || !ok(page[1])) {  // rows of pages that hold no token: their scales may be anything
+#pragma unroll
+            for (int c = 0; c < WAVES; ++c) {
+                const int first = at + 32 * c + 4 * (lane >> 4), end = at + 32 * c < k1 && ok(page[c / 2]) ? kvalid : 0;
+                uint32_t keep[2] = {0, 0};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) keep[j / 4] |= first + 16 * (j / 4) + j % 4 < end ? 0xffu << (8 * (j % 4)) : 0u;
+                vs[c] &= v4u{keep[0], keep[1], keep[0], keep[1]};
+            }
+        }
         // o += V^T P^T, 32 keys and 32 dims at a time; the next ones are converted between the products
         v4u ve[2], vo[2];  // one dim of two keys
         auto values = [&](int s) __attribute__((always_inline)) {
             const int c = s / 2;
-            if (s % 2 == 0) {
-                const int kc = at + 32 * c;
-                const bool vin = kc < k1 && ok(page[c / 2]);
-                if (!vin || kc + 32 > kvalid) {  // rows of the page that hold no token: their scales may be anything
-                    const int first = kc + 4 * (lane >> 4), end = vin ? kvalid : 0;
-                    uint32_t keep[2] = {0, 0};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        keep[j / 4] |= first + 16 * (j / 4) + j % 4 < end ? 0xffu << (8 * (j % 4)) : 0u;
-                    vs[c] &= v4u{keep[0], keep[1], keep[0], keep[1]};
-                }
-            }
             uint32_t w[8];
             values_of(v[c], vs[c], s % 2, w);
 #pragma unroll
@@ -792,40 +791,54 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a
             next[i] = page_of(at + 2 * STEP + PG * i);
         }
     }
-    // the rows' sums; the references are the same in all waves
+    // The rows' sums; the references are the same in all waves.  A wave passes its 64 dims of 16 rows at a time through its
+    // part of the query operands' LDS, so that 16 lanes load and store a row's 256 bytes.
+    constexpr int MS = 64 + 4;
+    float *mo = reinterpret_cast<float *>(lq) + wave * 16 * MS;
+    const int dim = 64 * wave + 4 * col;
+    size_t at[NRB][4];   // the lane's rows 16 j + 4 k + lane / 16: row of og
+    float4 z[NRB][4];    // and their gates, all requested before the first store
 #pragma unroll
     for (int j = 0; j < NRB; ++j) {
         const float ls = sum_quarters(sm[j].l);
         if (lane < 16) ll[wave][16 * j + lane] = ls;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = min(r0 + 16 * j + 4 * k + (lane >> 4), rows - 1), tok = r / a.grp;
+            at[j][k] = (size_t) (c0 + tok) * a.nq + g * a.grp + (r - tok * a.grp);
+            if (a.nsplit == 1) z[j][k] = *reinterpret_cast<const float4 *>(a.qg + (at[j][k] * 2 + 1) * HD + dim);
+        }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NRB; ++j) {
-        const int row = 16 * j + col, r = r0 + row;
-        if (r >= rows) continue;
-        const float L = (ll[0][row] + ll[1][row]) + (ll[2][row] + ll[3][row]);
-        const int tok = r / a.grp, d = 64 * wave + 8 * (lane >> 4);
-        const size_t out = (size_t) (c0 + tok) * a.nq + g * a.grp + (r - tok * a.grp);
-        const size_t part = (((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + row;
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees no key: zeros
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {  // four dims
-            const v4f e = o[j][t / 2][0], f = o[j][t / 2][1];
-            const int i = t % 2 * 2, dim = d + 32 * (t / 2) + 4 * (t % 2);
-            const float4 x = make_float4(e[i], f[i], e[i + 1], f[i + 1]);
+        for (int u = 0; u < 4; ++u) {
+            const v4f e = o[j][u / 2][0], f = o[j][u / 2][1];
+            const int i = u % 2 * 2;
+            *reinterpret_cast<float4 *>(mo + col * MS + 32 * (u / 2) + 8 * (lane >> 4) + 4 * (u % 2)) =
+                make_float4(e[i], f[i], e[i + 1], f[i + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int row = 16 * j + 4 * k + (lane >> 4);
+            const float4 x = *reinterpret_cast<const float4 *>(mo + (row - 16 * j) * MS + 4 * col);
+            if (r0 + row >= rows) continue;
+            const float L = (ll[0][row] + ll[1][row]) + (ll[2][row] + ll[3][row]);
             if (a.nsplit == 1) {
-                const float4 z = *reinterpret_cast<const float4 *>(a.qg + (out * 2 + 1) * HD + dim);
-                *reinterpret_cast<float4 *>(a.og + out * HD + dim) =
-                    make_float4(x.x * inv * sigmoidf_(z.x), x.y * inv * sigmoidf_(z.y), x.z * inv * sigmoidf_(z.z),
-                                x.w * inv * sigmoidf_(z.w));
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees no key: zeros
+                const float4 y = z[j][k];
+                *reinterpret_cast<float4 *>(a.og + at[j][k] * HD + dim) =
+                    make_float4(x.x * inv * gate_of(y.x), x.y * inv * gate_of(y.y), x.z * inv * gate_of(y.z),
+                                x.w * inv * gate_of(y.w));
             } else {
+                const size_t part = (((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + row;
                 *reinterpret_cast<float4 *>(a.part_o + part * HD + dim) = x;
+                if (dim == 0) a.part_ml[2 * part + 1] = L;
             }
         }
-        if (a.nsplit > 1 && wave == 0 && lane < 16) {
-            a.part_ml[2 * part] = sm[j].m;
-            a.part_ml[2 * part + 1] = L;
-        }
+        if (a.nsplit > 1 && wave == 0 && lane < 16 && r0 + 16 * j + lane < rows)
+            a.part_ml[2 * ((((size_t) item * a.nkv + g) * a.nsplit + sp) * RT + 16 * j + lane)] = sm[j].m;
     }
 }
 
@@ -861,7 +874,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
     float L = 0.0f;
     float4 o = f4(0.0f);
     auto join = [&](const float2 &x, const float4 &y) {
-        const float f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x.x - M) * SM_SCALE);
+        const float f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - M);
         L = fmaf(x.y, f, L);
         o = add_scaled(o, y, f);
     };
@@ -884,7 +897,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     reinterpret_cast<float4 *>(a.og + at * HD)[lane] = make_float4(
-        o.x * inv * sigmoidf_(z.x), o.y * inv * sigmoidf_(z.y), o.z * inv * sigmoidf_(z.z), o.w * inv * sigmoidf_(z.w));
+        o.x * inv * gate_of(z.x), o.y * inv * gate_of(z.y), o.z * inv * gate_of(z.z), o.w * inv * gate_of(z.w));
 }
 
 template <int RT> void launch(const Kv4Args &a, hipStream_t st) {

@@ -77,14 +77,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], v4u &hi, v4u &lo) {
 __device__ __forceinline__ int exp_of(float x) { return x > 0.0f ? max(-100, min(126, (int) (__float_as_uint(x) >> 23) - 127)) : 0; }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t) (e + 127) << 23); }
 
-// e^x = 2^t (1 + r log 2), t = x log2 e as rounded and r what the rounding left, with log2 e in two parts: off by less than
-// 2^-22 of the value.  0 below fp32's normal range; beyond it no finite value.
-__device__ __forceinline__ float exp_(float x) {
-    const float t = x * 1.44269504f, r = fmaf(x, 1.925963e-8f, fmaf(x, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * 0.693147181f, e);
-}
-// (bounded so that e^-x is finite: what x would make of it beyond is below 2^-120)
-__device__ __forceinline__ float silu_(float x) { return x * __builtin_amdgcn_rcpf(1.0f + exp_(fminf(-x, 88.0f))); }
+__device__ __forceinline__ float silu_(float x) { return x * gate_of(x); }
 
 __device__ __forceinline__ float4 lds4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 

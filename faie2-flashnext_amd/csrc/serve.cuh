@@ -38,4 +38,13 @@ __device__ __forceinline__ float sum_quarters(float x) {
     return r.x + r.y;
 }
 
+// e^x = 2^t (1 + r log 2), t = x log2 e as rounded and r what the rounding left, with log2 e in two parts: off by less than
+// 2^-22 of the value.  0 below fp32's normal range; beyond it no finite value.
+__device__ __forceinline__ float exp_(float x) {
+    const float t = x * 1.44269504f, r = fmaf(x, 1.925963e-8f, fmaf(x, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * 0.693147181f, e);
+}
+// 1 / (1 + e^-x), within 2^-21 of the value (bounded so that e^-x is finite: beyond, it is below 2^-126)
+__device__ __forceinline__ float gate_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_(fminf(-x, 88.0f))); }
+
 }  // namespace fn
