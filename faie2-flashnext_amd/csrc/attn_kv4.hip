@@ -361,6 +361,8 @@ struct Softmax {
 // eight lanes adds the halves.  P.V: the conversion leaves dims 2m, 2m + 1 of a key in one register, which as it stands
 // is two contraction slots; the columns 0..7 hold a probability in the first of them and 0 in the second, which gives
 // the even dims, and 8..15 the other way round.  So nothing is permuted and the sums take half the registers.
+// What bounds it: the cache's bytes at long contexts (64 requests of 8k keys: 289 MB in 69 us, 4.2 TB/s, while vector and
+// matrix instructions take half and two fifths of the cycles), latency at short ones (one request of 4k keys: 5.3 us).
 __global__ void __launch_bounds__(WAVES * 64, 3) k_attn_kv4(const Kv4Args a) {
     constexpr int RT = 8, MS = HD + 4;  // rows, floats a row of the merge
     constexpr int MB = WAVES * RT * MS * 4;
@@ -573,12 +575,14 @@ __device__ __forceinline__ int longest_first(const Kv4Args &a, int rt, int z, in
 
 // grid (nsplit, nkv, items), four waves: the 32 rows of an item against the keys of a split, 128 keys at a time.  For the
 // scores a wave takes 32 of the keys, for the values a quarter of the dims: so each value is converted once for all rows,
-// the sums of a wave are 32 registers and not 128 (which left one wave a SIMD: 463 us for what now takes 340), and nothing
+// the sums of a wave are 32 registers and not 128 (which left one wave a SIMD: 463 us for what now takes 323), and nothing
 // is left to be joined at the end.  The waves share the rows' references (a row's largest score goes through the LDS) and
 // the probabilities.
-// What bounds it: 136 matrix instructions of 16 cycles and some 600 vector instructions of 4 a wave and step, which two
-// waves a SIMD overlap in part, and 240 KB a step through the LDS.  A prompt of 4001 tokens, 16 + 2 heads: 340 us, the
-// matrix instructions alone 113 us; 24 requests of 1 or 300 tokens over 0.8k to 8k keys: 573 us, 197 us.
+// What bounds it: 136 matrix instructions of 16 cycles and some 570 vector instructions of 4 a wave and step, which two
+// waves a SIMD overlap in part, and 240 KB a step through the LDS: 8,100 to 8,700 cycles a step of two workgroups a CU, of
+// which the scores take 2,000, the largest scores 700, the probabilities 1,900 and the values 3,400.  A prompt of 4001
+// tokens, 16 + 2 heads: 323 us, the matrix instructions alone 113 us; 24 requests of 1 or 300 tokens over 0.8k to 8k keys:
+// 534 us, 197 us.
 __global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a) {
     constexpr int RT = 16 * NRB, STEP = WAVES * 32;
     __shared__ __align__(16) uint8_t lq[NRB * QBLK];
@@ -687,6 +691,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a
             FN_KV4_PART(0, 0);
             FN_KV4_PART(1, 0);
 #undef FN_KV4_PART
+            // (here, and not behind the branches of the first row block, where the compiler would move half of the products)
+#pragma unroll
+            for (int j = 0; j < NRB; ++j) asm volatile("" : "+v"(acc[0][j]), "+v"(acc[1][j]));
 #pragma unroll
             for (int j = 0; j < NRB; ++j)
 #pragma unroll
@@ -842,7 +849,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) k_attn_kv4_rows(const Kv4Args a
     }
 }
 
-// grid (items RT, nkv), four waves a row, lane = 4 dims: the splits of a row joined, and the gate
+// grid (items RT, nkv), four waves a row, lane = 4 dims: the splits of a row joined, and the gate.  A chain of latencies:
+// 2.8 us for 32 splits (3.6 us with the sums requested behind the references).
 template <int RT>
 __global__ void __launch_bounds__(256) k_kv4_combine(const Kv4Args a) {
     __shared__ float4 part[WAVES][HD / 4];
