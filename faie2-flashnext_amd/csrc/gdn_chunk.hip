@@ -12,7 +12,7 @@
 //   k_chunk_scan, one a (request, value head, columns of S), which walks the request's chunks with its columns of S in
 //     registers: three small products one after the other a chunk, and two exchanges through the LDS.
 // W and U0 are formed before the scan, not M inside it: the scan is the sequential part, and M there is one more product
-// and exchange a chunk (15k tokens, 32 value heads: scan 596 us with M, 405 us with W; the other kernel 252 and 272 us).
+// and exchange a chunk (15k tokens, 32 value heads: scan 596 us with M, 392 us with W; the other kernel 252 and 272 us).
 // Products: an fp32 operand is two f16 values (hi and lo, 11 bits each) under a power-of-two scale, and a product is hi
 // hi + hi lo + lo hi on v_mfma_f32_16x16x32_f16: what is left out is 2^-22 of a product at the worst and 2^-24 in the
 // mean, in half the instructions of six bf16 products and a fifth of the time of fp32 ones.  f16's range is met by
@@ -557,8 +557,8 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
 // Operands are requested a chunk ahead, each as soon as its registers are free, and between other work, because a wave
 // stops at a load that the address unit cannot take yet.  That reaches over the L2's latency, not the memory's, and the
 // workgroups of a head read the same operands at the same time.  So wave 8 touches the operands two chunks ahead, each of
-// the head's workgroups (which share an XCD where nvh is a multiple of 8) its part of the lines: 538 us without it, 405 us
-// with it at 15k tokens and 32 heads.
+// the head's workgroups (which share an XCD where nvh is a multiple of 8) its part of the lines: 538 us without it, 392 us
+// with it at 15k tokens and 32 heads.  (Loads to the LDS hold no registers, but a barrier waits for them: 402 us.)
 // What bounds it then: the way round the state waves, 1.3 us a chunk of 1.7: two barriers, two trips through the LDS and
 // the products between them; the rest is the operands' 113 KiB a chunk, whatever the columns, at 64 bytes a cycle and CU.
 // That is why two column tiles (2.7 us a chunk) are taken as soon as one would leave more workgroups than CUs.
@@ -630,22 +630,26 @@ __global__ void __launch_bounds__(576, 3) k_chunk_scan(const ChunkArgs a) {
         for (int n = 0; n < NC; ++n) acc[n] = (t[0][n] * si[0][n] + t[1][n] * si[1][n]) + (t[2][n] * si[2][n] + t[3][n] * si[3][n]);
     };
     if (role == 2) {
-        __shared__ uint32_t sink[64];  // loads to the LDS hold no registers; what they leave here is not read
+        constexpr int LINES = D / 16 / NC * 64, NH = (HEAD_BYTES / 128 + LINES - 1) / LINES, NK = (KEY_BYTES / 128 + LINES - 1) / LINES;
+        uint32_t x[NH + NK];
         auto touch = [&](int i) __attribute__((always_inline)) {
             const brsrc hd = head(i), kd = key(i);
-            auto *to = (__attribute__((address_space(3))) void *) sink;
-            for (int l = blockIdx.y * 64 + lane; l < HEAD_BYTES / 128; l += D / 16 / NC * 64)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(hd, to, 4, l * 128, 0, 0, 0);
-            for (int l = blockIdx.y * 64 + lane; l < KEY_BYTES / 128; l += D / 16 / NC * 64)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(kd, to, 4, l * 128, 0, 0, 0);
+            const int at = (blockIdx.y * 64 + lane) * 128;  // (lines behind the operands: not loaded)
+#pragma unroll
+            for (int k = 0; k < NH; ++k) x[k] = __builtin_amdgcn_raw_buffer_load_b32(hd, at + k * LINES * 128, 0, 0);
+#pragma unroll
+            for (int k = 0; k < NK; ++k) x[NH + k] = __builtin_amdgcn_raw_buffer_load_b32(kd, at + k * LINES * 128, 0, 0);
         };
         touch(min(1, chunks - 1));
         for (int i = 0; i < chunks; ++i) {
             lds_barrier();
+#pragma unroll
+            for (int k = 0; k < NH + NK; ++k) asm volatile("" ::"v"(x[k]));  // the last chunk's, which have come by now
             touch(min(i + 2, chunks - 1));
             lds_barrier();
         }
-        __builtin_amdgcn_s_waitcnt(0);  // the LDS is the workgroup's until they have come
+#pragma unroll
+        for (int k = 0; k < NH + NK; ++k) asm volatile("" ::"v"(x[k]));
     } else if (role == 0) {
         float s[NC][2][4];
         float *Sg = p.S + ((size_t) b * p.nvh + h) * D * D + col0 + r;
@@ -884,7 +888,7 @@ int gdn_chunk_launch(const GdnChunk &p, hipStream_t st) {
     a.keys = static_cast<uint8_t *>(p.work);
     a.heads = a.keys + items * p.nkh * KEY_BYTES;
     // columns a scan workgroup (above): one tile while every workgroup has a CU of its own.  48 value heads of one request:
-    // 277 us with one tile, 174 us with two; 32 value heads: 405 us with one (256 workgroups, 1.7 us a chunk), 2.7 us a
+    // 277 us with one tile, 174 us with two; 32 value heads: 392 us with one (256 workgroups, 1.7 us a chunk), 2.7 us a
     // chunk with two
     const int nc = (long long) p.B * p.nvh * (D / 16) > device_cus() ? 2 : 1;
     const dim3 gi((unsigned) items, p.nkh), gs(p.nvh, D / 16 / nc, p.B);
