@@ -353,3 +353,83 @@ def test_gdn_core_columns(fnlib, lens, nkh, nvh):
     e = oracle.relerr(d["o"].download(), o), oracle.relerr(d["S"].download(), rS)
     _say("o, S", e)
     assert max(e) <= TOL
+
+
+# more requests than a wave has lanes: a request is found in two steps, and items come in their own order
+# (with 16 query heads a kv head in items of 32 rows, with 8 in items of 8)
+@pytest.mark.parametrize("B,new,nsplit,nq", [(64, 4, 1, 16), (65, 4, 1, 16), (70, 5, 3, 16), (300, 4, 1, 16), (150, 1, 2, 8), (70, 4, 1, 8)])
+def test_attn_many_requests(fnlib, B, new, nsplit, nq):
+    _say("kv4 many", B, new, nq)
+    r = np.random.default_rng(B)
+    past, nnew = r.integers(0, 150, B).tolist(), [int(x) for x in r.integers(0 if new > 1 else 1, new + 1, B)]
+    c = _batch(past, nnew, nq, 1, sum(nnew) + 2, seed=B)
+    ref = {k: np.array(v, copy=True) for k, v in c.items()}
+    og, cache = _attn(fnlib, nsplit, **c)
+    want = serve.attn_kv4(*(ref[k] for k in ("past", "cu", "table", "slot", "qg", "k", "v", "wq", "wk", "cache")))
+    n = sum(nnew)
+    assert np.array_equal(cache, ref["cache"]) and (og[n:] == 7.5).all()
+    e = oracle.relerr(og[:n], want)
+    _say("og", e)
+    assert e <= TOL
+
+
+def test_gdn_core_many_requests(fnlib):
+    _say("core many")
+    r = np.random.default_rng(9)
+    n = lambda *s: r.standard_normal(s).astype(np.float32)  # noqa: E731
+    lens = r.integers(0, 80, 200)
+    lens[:5] = 0
+    B, T, nkh, nvh = len(lens), int(lens.sum()) + 3, 1, 2
+    unit = lambda x: x / np.linalg.norm(x, axis=-1, keepdims=True)  # noqa: E731
+    a = dict(q=unit(n(T, nkh, D)), k=unit(n(T, nkh, D)), v=n(T, nvh, D), beta=(1 / (1 + np.exp(-n(T, nvh)))).astype(np.float32),
+             g=(-np.log1p(np.exp(n(T, nvh)))).astype(np.float32))
+    S = 0.1 * n(B, nvh, D, D)
+    cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    d = {k: hiprt.Buf.like(v) for k, v in {"cu": cu, **a, "S": S, "o": np.full((T, nvh, D), 7.5, np.float32)}.items()}
+    wb = fnlib.gdn_chunk_work_bytes(B, T, nkh, nvh)
+    w = hiprt.Buf.like(np.full(wb, 255, np.uint8))
+    fnlib.gdn_core_chunk_dev(B, T, nkh, nvh, *(b.ptr for b in d.values()), w.ptr, wb)
+    hiprt.sync()
+    o, rS = np.zeros((cu[-1], nvh, D)), S.astype(np.float64)
+    for b in np.flatnonzero(lens):
+        x, Sb = slice(cu[b], cu[b + 1]), rS[b:b + 1].copy()
+        o[x] = oracle.gdn_core(*(np.ascontiguousarray(a[k][x])[None] for k in ("q", "k", "v", "beta", "g")), Sb)[0]
+        rS[b] = Sb[0]
+    got, gS = d["o"].download(), d["S"].download()
+    assert (got[cu[-1]:] == 7.5).all() and np.array_equal(gS[lens == 0], S[lens == 0])
+    e = oracle.relerr(got[:cu[-1]], o), oracle.relerr(gS, rS)
+    _say("o, S", e)
+    assert max(e) <= TOL
+
+
+def test_plan_and_release_of_the_most_requests(fnlib):
+    """8000 requests in one call, and all their pages back."""
+    _say("plan 8000")
+    r = np.random.default_rng(8)
+    B, mb = 8000, 4
+    past = r.integers(0, 190, B).astype(np.int32)
+    nnew = r.integers(0, 3, B).astype(np.int32)
+    T = int(nnew.sum()) + 1
+    have = (past + 63) // 64
+    npages = int(have.sum()) + 400
+    order = r.permutation(npages).astype(np.int32)
+    table = np.full((B, mb), -1, np.int32)
+    table[np.arange(mb)[None] < have[:, None]] = order[:have.sum()]
+    free = np.full(npages, -1, np.int32)
+    free[:400] = order[have.sum():]
+    z = lambda *s: np.zeros(s, np.int32)  # noqa: E731
+    d = {k: hiprt.Buf.like(a) for k, a in dict(past=past, nnew=nnew, free=free, top=np.array([400], np.int32), table=table, cu=z(B + 1),
+                                               slot=z(T), seq=z(T), done=z(B) + 1).items()}
+    fnlib.dev_status()
+    fnlib.page_plan_dev(B, T, mb, npages, d["past"].ptr, d["nnew"].ptr, d["free"].ptr, d["top"].ptr, d["top"].ptr, d["table"].ptr,
+                        d["cu"].ptr, d["slot"].ptr, d["seq"].ptr)
+    hiprt.sync()
+    ref = serve.plan(past, nnew, T, mb, free, 400, table)
+    for got, want in zip(("top", "table", "cu", "slot", "seq"), ref):
+        assert np.array_equal(d[got].download().reshape(np.shape(want)), want), got
+    d["past"].upload(past + nnew)
+    fnlib.page_release_dev(B, mb, npages, d["done"].ptr, d["past"].ptr, d["free"].ptr, d["top"].ptr, d["table"].ptr)
+    hiprt.sync()
+    assert fnlib.dev_status() == 0
+    assert d["top"].download()[0] == npages and np.array_equal(np.sort(d["free"].download()), np.arange(npages))
+    assert (d["table"].download() == -1).all() and not d["past"].download().any()
