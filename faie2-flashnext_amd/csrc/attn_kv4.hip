@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
             for (int i = 0; i < 32; ++i) {
                 const int d = 32 * gi + i, o = d < half ? d + half : d < a.nrot ? d - half : d;
                 x[i] = fmaf(qrow[wave][lane >> 3][o], sf[d], x[i] * cf[d]);
-                if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // reads of eight at a time: 128 registers, four waves a SIMD
+                if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (reads of eight at a time)
             }
         }
         __builtin_amdgcn_wave_barrier();

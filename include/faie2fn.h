@@ -294,7 +294,8 @@ int fn_test_attn_qsa(int B, int nq, int nkv, int hd, int nrot, float theta, floa
  * (free_left may be free_top: the stack then moves on; apart, the call can be repeated).  Written: cu [B + 1]; for each
  * of T rows slot [T] = page * 64 + row of the page and seq [T] = its request (-1 in rows from cu[B] on).  A block that
  * gets no page (none is left, or it lies past max_blocks) has table entry -1 (none past max_blocks) and its tokens slot
- * -1: not cached, and the status word says so.  New tokens beyond T rows are cut off.  B 1..8000. */
+ * -1: not cached, and the status word says so.  New tokens beyond T rows are cut off.  B 1..8000, T up to
+ * 2^30.  (A batch of more than 4096 rows takes one launch if free_left is not free_top, and two if it is.) */
 int fn_page_plan_dev(int B, int T, int max_blocks, int npages, const int32_t *past, const int32_t *nnew,
                      const int32_t *free_list, const int32_t *free_top, int32_t *free_left, int32_t *table, int32_t *cu,
                      int32_t *slot, int32_t *seq, void *stream);
@@ -325,6 +326,7 @@ int fn_kv4_unpack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, c
  * passed over; a query that finds no key gets zeros).  The rotation's angle is taken in 64 bits.  nq / nkv any whole number.
  * nsplit: key splits of a row (fn_attn_kv4_nsplit: the choice for contexts of up to ctx keys).  All arrays but the
  * int32 ones 16-byte aligned; work: fn_attn_kv4_work_bytes() bytes.  The slots of one call (other than -1) are different.
+ * T nq / nkv / 32 + B (in batches of up to 24 nkv / nq rows a request: / 8) is at most 65535.
  * Requests may name the same pages in their tables.  A row whose seq is not the request whose rows it lies in is not
  * cached, its output is undefined, and the status word says so. */
 int fn_attn_kv4_dev(int B, int T, int nq, int nkv, int hd, int nrot, float theta, float eps, int max_blocks, int npages,

@@ -433,3 +433,37 @@ def test_plan_and_release_of_the_most_requests(fnlib):
     assert fnlib.dev_status() == 0
     assert d["top"].download()[0] == npages and np.array_equal(np.sort(d["free"].download()), np.arange(npages))
     assert (d["table"].download() == -1).all() and not d["past"].download().any()
+
+
+# one workgroup for all tokens or many, with the count that is left in a place of its own and in the place that is read, and
+# requests whose past stays in the LDS or not
+@pytest.mark.parametrize("B,T,in_place", [(3, 4096, False), (3, 4097, False), (3, 4097, True), (40, 9000, False), (40, 9000, True),
+                                          (5000, 5003, False), (5001, 5003, False), (5001, 5003, True)])
+def test_plan_variants(fnlib, B, T, in_place):
+    _say("plan variants", B, T, in_place)
+    r = np.random.default_rng(T + B)
+    past = r.integers(0, 200, B).astype(np.int32)
+    past[1] = -3
+    nnew = np.bincount(r.integers(0, B, T - 2), minlength=B).astype(np.int32)
+    want = (np.maximum(past, 0) + nnew + 63) // 64
+    mb = int(want.max()) - 1 if B == 40 else int(want.max())    # (of 40 requests some have tokens past the table)
+    have = np.minimum((np.maximum(past, 0) + 63) // 64, mb)
+    npages = int(have.sum()) + int((want - have).sum()) - (5 if B == 40 else 0)    # (and some pages are missing)
+    order = r.permutation(npages).astype(np.int32)
+    table = np.full((B, mb), -1, np.int32)
+    table[np.arange(mb)[None] < have[:, None]] = order[:have.sum()]
+    top = npages - int(have.sum())
+    free = np.full(npages, -1, np.int32)
+    free[:top] = order[have.sum():]
+    z = lambda *s: np.zeros(s, np.int32) - 9  # noqa: E731
+    d = {k: hiprt.Buf.like(a) for k, a in dict(past=past, nnew=nnew, free=free, top=np.array([top], np.int32), left=z(1), table=table,
+                                               cu=z(B + 1), slot=z(T), seq=z(T)).items()}
+    left = d["top"] if in_place else d["left"]
+    fnlib.dev_status()
+    fnlib.page_plan_dev(B, T, mb, npages, d["past"].ptr, d["nnew"].ptr, d["free"].ptr, d["top"].ptr, left.ptr, d["table"].ptr,
+                        d["cu"].ptr, d["slot"].ptr, d["seq"].ptr)
+    hiprt.sync()
+    fnlib.dev_status()
+    ref = serve.plan(past, nnew, T, mb, free, top, table)
+    for got, want in zip((left, d["table"], d["cu"], d["slot"], d["seq"]), ref):
+        assert np.array_equal(got.download().reshape(np.shape(want)), want)

@@ -47,7 +47,8 @@ def test_unaligned_pointers_are_refused(fnlib, call, names):
 
 @pytest.mark.parametrize("call,match,bad", [
     ("page_plan_dev", "B must be", dict(B=0)), ("page_plan_dev", "B must be", dict(B=8001)),
-    ("page_plan_dev", "T must be", dict(T=0)), ("page_plan_dev", "max_blocks", dict(max_blocks=0)),
+    ("page_plan_dev", "T must be", dict(T=0)), ("page_plan_dev", "T must be", dict(T=(1 << 30) + 1)),
+    ("page_plan_dev", "max_blocks", dict(max_blocks=0)),
     ("page_plan_dev", "npages", dict(npages=0)), ("page_plan_dev", "npages", dict(npages=1 << 25)),
     ("page_release_dev", "B must be", dict(B=-1)), ("page_release_dev", "npages", dict(npages=1 << 25)),
     ("kv4_pack_dev", "n and nkv", dict(n=0)), ("kv4_pack_dev", "n and nkv", dict(nkv=0)),
