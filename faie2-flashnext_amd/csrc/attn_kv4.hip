@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
     __shared__ float qrow[PART == PREP_KEYS ? 1 : WAVES][8][MAXROT + 4];
     const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     // the wave's first rows, and what else depends on no other load, are requested before anything that waits
-    const int slot = a.slot[t], half = a.nrot / 2;
+    const int slot = a.slot[t], b = a.seq[t], total = min(a.cu[a.B], a.T), half = a.nrot / 2;
     auto freq = [&](int d) { return a.freq[d < half ? d : d < a.nrot ? d - half : 0]; };
     double fr = freq(threadIdx.x);
     const int waves = blockDim.x >> 6, octets = (a.nq + 7) / 8;
@@ -110,15 +110,15 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
         }
     };
     if (first < tasks) request(first);
-    const int total = min(a.cu[a.B], a.T);
     if (t >= total) return;
-    const int b = a.seq[t];
-    if (b < 0 || b >= a.B || t < a.cu[b] || t >= a.cu[b + 1] || a.cu[b] < 0) {
+    // (three loads at once, of some request where seq names none)
+    const int sb = min(max(b, 0), a.B - 1), c0 = a.cu[sb], c1 = a.cu[sb + 1], past = a.past[sb];
+    if (b != sb || t < c0 || t >= c1 || c0 < 0) {
         if (threadIdx.x == 0) atomicOr(a.status, FN_STATUS_ROWS);
         return;
     }
-    const long long P = (long long) a.past[b] + (t - a.cu[b]);
-    if ((a.past[b] < 0 || P >= (long long) a.mb * PG) && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_POS);
+    const long long P = (long long) past + (t - c0);
+    if ((past < 0 || P >= (long long) a.mb * PG) && threadIdx.x == 0) atomicOr(a.status, FN_STATUS_POS);
     // the angle in 64 bits: a float product is off by up to half a radian at a million tokens
     for (int d = threadIdx.x; d < MAXROT; d += blockDim.x) {
         double sv = 0.0, cv = 1.0;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
         const uint32_t u = __float_as_uint(am);
         int e0 = (int) (u >> 23) - 127 - 2 + ((u & 0x7fffffu) > 0x700000u);
         e0 = max(e0, EMIN);
-        const int g = h / a.grp, row = (t - a.cu[b]) * a.grp + (h - g * a.grp);
+        const int g = h / a.grp, row = (t - c0) * a.grp + (h - g * a.grp);
         const int item = first_item(a.cu, b, a.grp, RT) + row / RT;
         uint8_t *dst = a.Q + ((size_t) g * a.items + item) * item_bytes<RT> + (RT == 8 ? 0 : row % RT / 16 * QBLK);
         const int uh = gi >> 2, ln = (gi & 3) * 16 + row % (RT == 8 ? 8 : 16);
