@@ -96,12 +96,19 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
     __shared__ double G[C];
     const GdnChunk &p = a.p;
     const int item = blockIdx.x, kh = blockIdx.y;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     int r = lane & 15, q4 = lane >> 4;
     const int b = request_of(p.cu, p.B, item, 1, C);
     const int c0 = p.cu[b], t0 = (item - first_item(p.cu, b, 1, C)) * C, n = min(C, min(p.cu[b + 1], p.T) - c0 - t0);
     if (c0 < 0 || t0 < 0 || n <= 0) return;
     const size_t row0 = (size_t) c0 + t0;
+    // 16-row tiles that hold a token: of the others no row operand is written (the descriptor is empty), or read
+    const int tiles = __builtin_amdgcn_readfirstlane((n + 15) / 16);
+    // (the place is in the descriptor and not in a scalar offset: behind a store of 16 bytes with one this compiler may
+    // write the store's registers in the next instruction, and the store was seen to take the new values)
+    auto put = [&](uint8_t *to, bool on, const v4u &x) __attribute__((always_inline)) {
+        __builtin_amdgcn_raw_buffer_store_b128(x, buf(to, on ? FRAG : 0), lane * 16, 0, 0);
+    };
     uint8_t *kd = a.keys + ((size_t) item * p.nkh + kh) * KEY_BYTES;
 
     const int per = p.nvh / p.nkh, Cc = 2 * p.nkh * D + p.nvh * D;
@@ -187,9 +194,8 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                     split8(v, kh_[s], kl[s]);
                 } else {
                     split8(v, qh[s], ql[s]);
-                    uint8_t *d = kd + QF + ((wave * 4 + s) * 2) * FRAG + lane * 16;
-                    *reinterpret_cast<v4u *>(d) = qh[s];
-                    *reinterpret_cast<v4u *>(d + FRAG) = ql[s];
+                    put(kd + QF + ((wave * 4 + s) * 2) * FRAG, wave < tiles, qh[s]);
+                    put(kd + QF + ((wave * 4 + s) * 2 + 1) * FRAG, wave < tiles, ql[s]);
                 }
             }
         }
@@ -339,9 +345,8 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                     for (int j = 0; j < 8; ++j) v[j] = pv[2 * s + j / 4][j % 4] * m;
                     v4u hi, lo;
                     split8(v, hi, lo);
-                    uint8_t *d = hd + PF + ((wave * 2 + s) * 2) * FRAG + lane * 16;
-                    *reinterpret_cast<v4u *>(d) = hi;
-                    *reinterpret_cast<v4u *>(d + FRAG) = lo;
+                    put(hd + PF + ((wave * 2 + s) * 2) * FRAG, wave < tiles, hi);
+                    put(hd + PF + ((wave * 2 + s) * 2 + 1) * FRAG, wave < tiles, lo);
                 }
         }
         // values of the wave's columns 32 wave + 16 c + l%16 (slots as in k^T)
@@ -483,7 +488,7 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
                 const float4 bk = lds4(&mback[1][16 * i + 4 * q4]);
                 const float4 o = make_float4(u[0] * bk.x * f, u[1] * bk.y * f, u[2] * bk.z * f, u[3] * bk.w * f);
                 um = fmaxf(um, fmaxf(fmaxf(fabsf(o.x), fabsf(o.y)), fmaxf(fabsf(o.z), fabsf(o.w))));
-                *reinterpret_cast<float4 *>(hd + U0 + ((i * 8 + 2 * wave + c) * 64 + lane) * 16) = o;
+                put(hd + U0 + (i * 8 + 2 * wave + c) * FRAG, i < tiles, __builtin_bit_cast(v4u, o));
             }
             um = max_quarters(um);
             if (q4 == 0) gd[G_UM + 32 * wave + 16 * c + r] = um;
@@ -536,9 +541,8 @@ __global__ void __launch_bounds__(256, 2) k_chunk_intra(const ChunkArgs a) {
             for (int j = 0; j < 8; ++j) x[j] = w[j / 4][i][j % 4] * m;
             v4u hi, lo;
             split8(x, hi, lo);
-            uint8_t *d = hd + WF + ((i * 4 + wave) * 2) * FRAG + lane * 16;
-            *reinterpret_cast<v4u *>(d) = hi;
-            *reinterpret_cast<v4u *>(d + FRAG) = lo;
+            put(hd + WF + ((i * 4 + wave) * 2) * FRAG, i < tiles, hi);
+            put(hd + WF + ((i * 4 + wave) * 2 + 1) * FRAG, i < tiles, lo);
             if (wave == 0 && q4 == 0) gd[G_W + t] = pow2(e);
         }
         if (wave == 1) {
@@ -580,11 +584,14 @@ __global__ void __launch_bounds__(576, 3) k_chunk_scan(const ChunkArgs a) {
     const int tok = 16 * wave + 4 * q4;  // the lane's first token
     const uint32_t lane16 = lane * 16;
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto key = [&](int i) __attribute__((always_inline)) {
-        return buf(a.keys + ((size_t) (item0 + i) * p.nkh + kh) * KEY_BYTES, KEY_BYTES);
+    // the chunk's operands.  Of a 16-row tile that holds no token the row operands were not written: the descriptor is
+    // empty then, and loads give zeros.
+    auto holds = [&](int i) { return 16 * wave < len - i * C; };
+    auto key = [&](int i, bool on = true) __attribute__((always_inline)) {
+        return buf(a.keys + ((size_t) (item0 + i) * p.nkh + kh) * KEY_BYTES, on ? KEY_BYTES : 0);
     };
-    auto head = [&](int i) __attribute__((always_inline)) {
-        return buf(a.heads + ((size_t) (item0 + i) * p.nvh + h) * HEAD_BYTES, HEAD_BYTES);
+    auto head = [&](int i, bool on = true) __attribute__((always_inline)) {
+        return buf(a.heads + ((size_t) (item0 + i) * p.nvh + h) * HEAD_BYTES, on ? HEAD_BYTES : 0);
     };
     auto ld = [&](brsrc d, int at) __attribute__((always_inline)) {
         return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(d, (int) lane16, at, 0));
@@ -634,11 +641,20 @@ __global__ void __launch_bounds__(576, 3) k_chunk_scan(const ChunkArgs a) {
         uint32_t x[NH + NK];
         auto touch = [&](int i) __attribute__((always_inline)) {
             const brsrc hd = head(i), kd = key(i);
-            const int at = (blockIdx.y * 64 + lane) * 128;  // (lines behind the operands: not loaded)
+            const int n = len - i * C, l0 = blockIdx.y * 64 + lane;
+            // lines behind the operands, or of a tile without a token: not loaded
+            auto at = [&](int l, int tile) { return 16 * tile < n ? l * 128 : HEAD_BYTES; };
 #pragma unroll
-            for (int k = 0; k < NH; ++k) x[k] = __builtin_amdgcn_raw_buffer_load_b32(hd, at + k * LINES * 128, 0, 0);
+            for (int k = 0; k < NH; ++k) {
+                const int l = l0 + k * LINES, by = l * 128;
+                x[k] = __builtin_amdgcn_raw_buffer_load_b32(
+                    hd, at(l, by < PF ? by % U0 / (8 * FRAG) : by < GATES ? (by - PF) / (4 * FRAG) : 0), 0, 0);
+            }
 #pragma unroll
-            for (int k = 0; k < NK; ++k) x[NH + k] = __builtin_amdgcn_raw_buffer_load_b32(kd, at + k * LINES * 128, 0, 0);
+            for (int k = 0; k < NK; ++k) {
+                const int l = l0 + k * LINES, by = l * 128;
+                x[NH + k] = __builtin_amdgcn_raw_buffer_load_b32(kd, at(l, by < KT ? by / (8 * FRAG) : 0), 0, 0);
+            }
         };
         touch(min(1, chunks - 1));
         for (int i = 0; i < chunks; ++i) {
@@ -695,9 +711,9 @@ __global__ void __launch_bounds__(576, 3) k_chunk_scan(const ChunkArgs a) {
             reinterpret_cast<v2u *>(&op[wave / 2][n][1][lane])[wave & 1] = v2u{lo[0], lo[1]};
         };
         // in the order of the loop's requests: its waits count them as both ways into it have them
-        load_u0(head(0));
+        load_u0(head(0, holds(0)));
         __builtin_amdgcn_sched_barrier(0);
-        load_rows(head(0), WF, wf);
+        load_rows(head(0, holds(0)), WF, wf);
         __builtin_amdgcn_sched_barrier(0);
         load_kt(key(0));
         __builtin_amdgcn_sched_barrier(0);
@@ -705,7 +721,7 @@ __global__ void __launch_bounds__(576, 3) k_chunk_scan(const ChunkArgs a) {
         for (int i = 0; i < chunks; ++i) {
             const int nx = min(i + 1, chunks - 1);
             const float *gd = gates[i & 1];
-            const brsrc hn = head(nx), kn = key(nx);
+            const brsrc hn = head(nx, holds(nx)), kn = key(nx);
             lds_barrier();  // S (and the largest values of the columns) is there
             const float4 sc = lds4(gd + G_SC);
             float si[4][NC], ub[NC];
@@ -779,15 +795,15 @@ __global__ void __launch_bounds__(576, 3) k_chunk_scan(const ChunkArgs a) {
         };
         load_gates(head(0));
         put_gates(0);
-        load_rows(key(0), QF, qf);
+        load_rows(key(0, holds(0)), QF, qf);
         __builtin_amdgcn_sched_barrier(0);
-        load_p(head(0));
+        load_p(head(0, holds(0)));
         __builtin_amdgcn_sched_barrier(0);
         for (int i = 0; i < chunks; ++i) {
             const int nx = min(i + 1, chunks - 1);
             const float *gd = gates[i & 1];
-            const brsrc hn = head(nx), kn = key(nx);
-            load_gates(hn);
+            const brsrc hn = head(nx, holds(nx)), kn = key(nx, holds(nx));
+            load_gates(head(nx));
             lds_barrier();  // S (and the largest values of the columns) is there
             float si[4][NC], ub[NC];
             bounds(gd, gd[G_SC], si, ub);
