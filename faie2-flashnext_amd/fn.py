@@ -467,7 +467,8 @@ class FN:
         self.check(self.d.fn_attn_kv4_dev(B, T, nq, nkv, hd, nrot, float(theta), float(eps), max_blocks, npages, past, cu,
                                           table, slot, seq, qg, k, v, wq, wk, cache, nsplit, work, work_bytes, og, stream))
 
-    def gdn_chunk_work_bytes(self, B, T, nkh, nvh):
+    def gdn_chunk_work_bytes(self, B, T, nkh, nvh, block=False):
+        """Workspace bytes of gdn_core_chunk_dev, or with block of gdn_block_chunk_dev: one size serves both."""
         return int(self.d.fn_gdn_chunk_work_bytes(B, T, nkh, nvh))
 
     def gdn_core_chunk_dev(self, B, T, nkh, nvh, cu, q, k, v, beta, g, S, o, work, work_bytes, stream=0, dk=128, dv=128,
