@@ -235,7 +235,7 @@ def prepare(case, seed):
         s["nsplit"] = L.attn_kv4_nsplit(s["B"], s["T"], c["nq"], c["nkv"], max(p + n for p, n in zip(past, new)))
         s["wb"] = L.attn_kv4_work_bytes(s["B"], s["T"], c["nq"], c["nkv"], s["nsplit"])
     elif own and c["kind"] != "plan":
-        s["wb"] = lib().gdn_chunk_work_bytes(s["B"], s["T"], c["nkh"], c["nvh"])
+        s["wb"] = lib().gdn_chunk_work_bytes(s["B"], s["T"], c["nkh"], c["nvh"], c["kind"] == "block")
     if "wb" in s:
         s["work"] = torch.empty(max(16, s["wb"]), dtype=torch.uint8, device=DEV)
     s["lengths"] = (past, new)
