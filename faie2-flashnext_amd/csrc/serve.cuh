@@ -39,12 +39,19 @@ __device__ __forceinline__ float sum_quarters(float x) {
 }
 
 // e^x = 2^t (1 + r log 2), t = x log2 e as rounded and r what the rounding left, with log2 e in two parts: off by less than
-// 2^-22 of the value.  0 below fp32's normal range; beyond it no finite value.
+// 2^-22 of the value.  For |x| up to 1e38, whose t is finite: 0 where e^x is below fp32's normal range, and from EXP_INF on
+// no finite value (a NaN where r is negative).
 __device__ __forceinline__ float exp_(float x) {
     const float t = x * 1.44269504f, r = fmaf(x, 1.925963e-8f, fmaf(x, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
     return fmaf(e, r * 0.693147181f, e);
 }
-// 1 / (1 + e^-x), within 2^-21 of the value (bounded so that e^-x is finite: beyond, it is below 2^-126)
-__device__ __forceinline__ float gate_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_(fminf(-x, 88.0f))); }
+// the least x with t = 128 or more, where 2^t is infinite; r is 3.5e-7 there, so that e^x is too
+constexpr float EXP_INF = 0x1.62e43p+6f;  // 88.72284
+// 1 / (1 + e^-x) of any x, within 2^-21 of the value; 0 where it is below fp32's normal range.  The argument is held in the
+// range of exp_ by a minimum and a maximum that keep a NaN (fminf and fmaxf drop it).
+__device__ __forceinline__ float gate_of(float x) {
+    const float y = __builtin_elementwise_minimum(__builtin_elementwise_maximum(-x, -88.0f), EXP_INF);
+    return __builtin_amdgcn_rcpf(1.0f + exp_(y));
+}
 
 }  // namespace fn

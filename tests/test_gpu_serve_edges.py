@@ -1,0 +1,108 @@
+"""GPU checks at the edges of the packed-batch operators: values that are not finite or hardly so, batches that are a part of
+a larger one, and what the status word says."""
+
+import numpy as np
+import pytest
+
+import oracle
+from oracle import serve
+from test_gpu_gdn_chunk import Block
+from test_gpu_serve import TOL, Batch, _run, _say
+
+pytestmark = pytest.mark.gpu
+
+# arguments of a gate: not finite, near the ends of fp32, around the place where e^-x leaves fp32 (88.72), ordinary
+GATES = np.array([np.nan, np.inf, -np.inf, 3e38, -3e38, 2.4e38, -2.4e38, 1e38, -1e38, 1e5, -1e5, 104, -104, 89, -89, 88.73, -88.73,
+                  88.7228, -88.7228, 88, -88, 87, -87, 20, -20, 1, -1, 0, -0.0], np.float32)
+
+
+def _sigmoid(x):
+    with np.errstate(over="ignore"):
+        return 1.0 / (1.0 + np.exp(-np.asarray(x, np.float64)))
+
+
+def _same(got, value, gate, what):
+    """NaN where value * gate is, infinities alike, and within 1e-5 of it.  A gate below 2^-126 (a denormal of fp32) may be
+    taken for 0, which moves the product by at most 2^-126 |value|; a product below 2^-126 may be too."""
+    with np.errstate(invalid="ignore"):
+        want = np.asarray(value, np.float64) * gate
+    with np.errstate(over="ignore"):
+        held = want.astype(np.float32)
+    assert np.array_equal(np.isnan(got), np.isnan(held)), what
+    inf = np.isinf(held)
+    assert np.array_equal(got[inf], held[inf]), what
+    f = np.isfinite(held)
+    bad = np.abs(got[f] - want[f]) > TOL * np.abs(want[f]) + 2.0 ** -126 * (1.0 + np.abs(value[f]))
+    assert not bad.any(), (what, got[f][bad][:5], want[f][bad][:5])
+
+
+# an item of 8 rows and of 32, each with its keys in one split (the walk applies the gate) and in several (the join does)
+@pytest.mark.parametrize("past,nnew", [([70, 3], [1, 1]), ([40, 0], [20, 9])])
+@pytest.mark.parametrize("nsplit", [1, 3])
+def test_attn_gate_of_any_value(fnlib, past, nnew, nsplit):
+    """The output is what it is under a gate of 1/2, times twice the sigmoid of the gate, whatever that is."""
+    _say("kv4 gate", past, nnew, nsplit)
+    c = Batch(past, nnew, nq=8, nkv=1, seed=31)
+    c.qg[:, :, 1] = 0
+    half, cache = _run(fnlib, c, nsplit)
+    assert np.isfinite(half).all()
+    gate = c.qg[:, :, 1]
+    gate[...] = np.resize(GATES, gate.shape)
+    og, again = _run(fnlib, c, nsplit)
+    assert np.array_equal(cache, again)
+    _same(og, 2.0 * half.astype(np.float64), _sigmoid(gate), "og")
+
+
+@pytest.mark.parametrize("gate_act", [0, 1])
+def test_block_gate_of_any_value(fnlib, gate_act):
+    """The same for the block's z: the output under a gate of 1/2 times 2 sigmoid(z), or 2 z sigmoid(z)."""
+    _say("block gate", gate_act)
+    c = Block([0, 9], [70, 3], seed=32, gate_act=0)
+    c.z[:] = 0
+    half = c.run(fnlib)[0].astype(np.float64)
+    assert np.isfinite(half).all()
+    c.gate_act = gate_act
+    c.z[...] = np.resize(GATES, c.z.shape)
+    value = 2.0 * half * (c.z.astype(np.float64) if gate_act else 1.0)
+    out = c.run(fnlib)[0]
+    # (a product beyond fp32 on its way to a finite value may be infinite there)
+    keep = (np.abs(value) < 1e37) | ~np.isfinite(value)
+    _same(out[keep], value[keep], _sigmoid(c.z)[keep], "out")
+
+
+@pytest.mark.parametrize("at", ["q", "k", "v"])
+@pytest.mark.parametrize("x", [-100.0, -1e5, -1e38, -3e38])
+def test_block_channels_far_below_zero(fnlib, at, x):
+    """SiLU of a conv output far below zero is 0, and the head goes on as with a 0 there."""
+    _say("block channel", at, x)
+    c = Block([0, 9], [70, 3], seed=33)
+    ch = {"q": 5, "k": c.nkh * 128 + 130, "v": 2 * c.nkh * 128 + 300}[at]
+    c.conv_w[ch] = [0, 0, 0, 1]
+    c.qkv[3::7, ch] = x
+    out, S, _ = c.run(fnlib)
+    ro, rS, _ = c.reference()
+    e = oracle.relerr(out, ro), oracle.relerr(S, rS)
+    _say("out, S", e)
+    assert max(e) <= TOL
+
+
+@pytest.mark.parametrize("x", [np.nan, np.inf, -np.inf])
+def test_block_channels_not_finite(fnlib, x):
+    """A value channel that is not finite leaves no finite output in its head from its token on, and reaches neither other
+    heads nor other requests nor earlier chunks."""
+    _say("block not finite", x)
+    c = Block([0, 9], [140, 20], seed=34)
+    ref, rS, _ = c.reference()
+    head, t = 2, 100
+    ch = 2 * c.nkh * 128 + head * 128 + 7
+    c.conv_w[ch] = [0, 0, 0, 1]
+    ref, rS, _ = c.reference()
+    c.qkv[t, ch] = x
+    out, S, _ = c.run(fnlib)
+    out, ref = out.reshape(c.T, c.nvh, 128), ref.reshape(c.T, c.nvh, 128)
+    assert not np.isfinite(out[t:140, head, 7]).any()
+    keep = np.ones((c.T, c.nvh), bool)
+    keep[64:140, head] = False
+    assert oracle.relerr(out[keep], ref[keep]) <= TOL
+    heads = [h for h in range(c.nvh) if h != head]
+    assert oracle.relerr(S[0, heads], rS[0, heads]) <= TOL and oracle.relerr(S[1], rS[1]) <= TOL
