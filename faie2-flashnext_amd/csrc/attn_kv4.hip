@@ -280,7 +280,10 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 }
 constexpr float SM_SCALE = 0.0625f * 1.4426950408889634f;  // 1 / sqrt(HD), and the softmax in powers of two
 constexpr float SLACK = 8.0f;                              // growth of a row's largest score, in powers of two, that moves its reference
-constexpr float PUP = 16.0f;                               // probabilities times 2^16: the parts of the least ones stay normal
+// Probabilities times 2^PUP, so that the sums hold every value of the format: the largest, 6 2^125, times probabilities of up
+// to 2^(SLACK + 1/2) over 2^19 keys stays below 2^128, and of the least, 2^-101, a product keeps 2^-149 (the matrix
+// instructions hold denormals), 20 bits of it.  (With 2^16 values from 2^103 on gave infinities.)
+constexpr float PUP = -28.0f;
 
 // 64 dims of the lane's eight keys as bf16 pairs: dims 32 t + 2 (l % 16), + 1
 __device__ __forceinline__ void values_of(const v4u &v, const v4u &vs, int t, uint32_t (&x)[8]) {

@@ -324,6 +324,8 @@ int fn_kv4_unpack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, c
  * past[b] + t - cu[b]: its normalised, rotated key and its value are written to slot[t] in 4 bits; its queries attend
  * the request's keys up to its own position as the cache holds them (a block whose table entry is outside the cache is
  * passed over; a query that finds no key gets zeros).  The rotation's angle is taken in 64 bits.  nq / nkv any whole number.
+ * Sums are in fp32: of any values of the cache over up to 2^19 keys of a query, of values below 2^117 over any number.  A score
+ * q.k that fp32 does not hold (packed keys near its end) may make the output NaN.
  * nsplit: key splits of a row (fn_attn_kv4_nsplit: the choice for contexts of up to ctx keys).  All arrays but the
  * int32 ones 16-byte aligned; work: fn_attn_kv4_work_bytes() bytes.  The slots of one call (other than -1) are different.
  * T nq / nkv / 32 + B (in batches of up to 24 nkv / nq rows a request: / 8) is at most 65535.

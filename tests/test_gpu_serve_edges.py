@@ -106,3 +106,52 @@ def test_block_channels_not_finite(fnlib, x):
     assert oracle.relerr(out[keep], ref[keep]) <= TOL
     heads = [h for h in range(c.nvh) if h != head]
     assert oracle.relerr(S[0, heads], rS[0, heads]) <= TOL and oracle.relerr(S[1], rS[1]) <= TOL
+
+
+# items of 8 and of 32 rows
+ITEMS = [([300, 70], [1, 1]), ([200, 0], [3, 60])]
+
+
+@pytest.mark.parametrize("past,nnew", ITEMS)
+@pytest.mark.parametrize("e", [-99, -60, 60, 100, 125])
+def test_attn_values_of_any_size(fnlib, past, nnew, e):
+    """Values times 2^e, from the least that the format holds whole to its largest: the same codes, and the outputs times 2^e.
+    (A product of the least value, 2^-101, and a probability is 2^-129 in the sums and rounds three times at 2^-150: 2^-19.4
+    of it, within the bar.)"""
+    _say("kv4 values", past, e)
+    c = Batch(past, nnew, nq=8, nkv=1, seed=35)
+    for b, p in enumerate(c.past):
+        for i in range(p):
+            s = int(c.full[b, i // 64]) * 64 + i % 64
+            K, V = serve.load(c.cache, [s])
+            serve.store(c.cache, s, K[0], np.ldexp(V[0], e))
+    c.v = np.ldexp(c.v, e)
+    ref = serve.attn_kv4(c.past, c.cu, c.full, c.slot, c.qg, c.k, c.v, c.wq, c.wk, c.cache.copy())
+    for nsplit in (1, 3):
+        og, _ = _run(fnlib, c, nsplit)
+        r = oracle.relerr(np.ldexp(og.astype(np.float64), -e), np.ldexp(ref, -e))
+        _say("og", nsplit, r)
+        assert r <= TOL
+
+
+@pytest.mark.parametrize("nnew", [1, 9])
+def test_attn_largest_values_under_growing_scores(fnlib, nnew):
+    """The largest value that the format holds in every place, under scores that grow by the most that a sum's reference lets
+    pass (8.48 powers of two): the output is that value times the gate."""
+    _say("kv4 largest", nnew)
+    past, top = 5000, 6.0 * 2.0 ** 125
+    c = Batch([past], [nnew], nq=8, nkv=1, seed=36)
+    c.qg[:, :, 0], c.wq[:], c.wk[:] = 1, 0.98, 0.375      # queries of 0.98 in every dim; the new keys are 0.375
+    c.k[:], c.v[:] = 1, top
+    rows = {}
+    for x in (0.0, 0.375):                                # 256 * 0.375 * 0.98 / 16 * log2(e) = 8.48
+        one = np.zeros((1, 1, serve.HEAD_BYTES), np.uint8)
+        for i in range(64):
+            serve.store(one, i, np.full((1, 256), x), np.full((1, 256), top))
+        rows[x] = one[0]
+    for i in range(serve.pages(past)):
+        c.cache[c.full[0, i]] = rows[0.0 if i < 8 else 0.375]
+    for nsplit in (1, 3):
+        og, _ = _run(fnlib, c, nsplit, nrot=0)
+        want = top * _sigmoid(c.qg[:, :, 1])
+        assert np.isfinite(og).all() and np.abs(og / want - 1).max() <= TOL
