@@ -857,7 +857,8 @@ __global__ void __launch_bounds__(256) k_chunk_finish(const ChunkArgs a, unsigne
     }
     const size_t row = (size_t) blockIdx.x * 8 + (threadIdx.x >> 5);
     const int l = threadIdx.x & 31;
-    const bool on = row < (size_t) min(p.cu[p.B], p.T) * p.nvh;
+    // rows before the first request are no request's, as those behind the last
+    const bool on = row >= (size_t) max(p.cu[0], 0) * p.nvh && row < (size_t) max(min(p.cu[p.B], p.T), 0) * p.nvh;
     const size_t at = on ? row * (D / 4) + l : 0;
     const float4 o = reinterpret_cast<const float4 *>(p.o)[at], z = reinterpret_cast<const float4 *>(p.z)[at];
     const float4 w = reinterpret_cast<const float4 *>(p.norm_w)[l];

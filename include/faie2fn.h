@@ -280,7 +280,8 @@ int fn_test_attn_qsa(int B, int nq, int nkv, int hd, int nrot, float theta, floa
 /* ======================================================================================================
  * 3c. Serving a packed batch (new; no counterpart in the reference, which decodes one sequence): requests of different
  *     lengths in one call.  Request b's new tokens are rows cu[b] .. cu[b + 1] - 1 of every per-token array of T rows; rows
- *     from cu[B] on are left as they were.  past [B] are the tokens that each request already has (0 for a new one).
+ *     before cu[0] and from cu[B] on are left as they were (a call may take a run of a batch's requests: cu + i, and the
+ *     arrays of B entries from i on, seq counted from i).  past [B] are the tokens that each request already has (0 for a new one).
  *     Nothing is allocated and no memset is recorded; a call can be captured into a graph and replayed with new
  *     contents of its buffers.  A workspace holds nothing between calls; calls that may run at the same time (two streams,
  *     two graphs) need one each.  All buffers are on the device that is current at the call.  cu does not decrease.  What

@@ -155,3 +155,15 @@ def test_attn_largest_values_under_growing_scores(fnlib, nnew):
         og, _ = _run(fnlib, c, nsplit, nrot=0)
         want = top * _sigmoid(c.qg[:, :, 1])
         assert np.isfinite(og).all() and np.abs(og / want - 1).max() <= TOL
+
+
+def test_block_of_a_part_of_a_batch(fnlib):
+    """The call of the requests from the second on (cu does not start at 0): the first one's rows, state and ring are left as
+    they were, the others have the bits of the call of all."""
+    _say("block part")
+    c = Block([4, 0, 9], [5, 70, 3], seed=37, pad=2)
+    out, S, conv = c.run(fnlib)
+    c.B, c.lens, c.cu, c.pos, c.S, c.conv = 2, c.lens[1:], c.cu[1:].copy(), c.pos[1:].copy(), c.S[1:].copy(), c.conv[1:].copy()
+    part, pS, pconv = c.run(fnlib)
+    assert (part[:5] == 7.5).all() and (part[78:] == 7.5).all()
+    assert np.array_equal(part[5:78], out[5:78]) and np.array_equal(pS, S[1:]) and np.array_equal(pconv, conv[1:])
