@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
     __shared__ float qrow[PART == PREP_KEYS ? 1 : WAVES][8][MAXROT + 4];
     const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     // the wave's first rows, and what else depends on no other load, are requested before anything that waits
-    const int slot = a.slot[t], b = a.seq[t], total = min(a.cu[a.B], a.T), half = a.nrot / 2;
+    const int slot = a.slot[t], b = a.seq[t], begin = a.cu[0], total = min(a.cu[a.B], a.T), half = a.nrot / 2;
     auto freq = [&](int d) { return a.freq[d < half ? d : d < a.nrot ? d - half : 0]; };
     double fr = freq(threadIdx.x);
     const int waves = blockDim.x >> 6, octets = (a.nq + 7) / 8;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256, PART == PREP_KEYS ? 6 : 2) k_kv4_prep(con
         }
     };
     if (first < tasks) request(first);
-    if (t >= total) return;
+    if (t < begin || t >= total) return;
     // (three loads at once, of some request where seq names none)
     const int sb = min(max(b, 0), a.B - 1), c0 = a.cu[sb], c1 = a.cu[sb + 1], past = a.past[sb];
     if (b != sb || t < c0 || t >= c1 || c0 < 0) {

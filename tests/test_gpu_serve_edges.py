@@ -167,3 +167,23 @@ def test_block_of_a_part_of_a_batch(fnlib):
     part, pS, pconv = c.run(fnlib)
     assert (part[:5] == 7.5).all() and (part[78:] == 7.5).all()
     assert np.array_equal(part[5:78], out[5:78]) and np.array_equal(pS, S[1:]) and np.array_equal(pconv, conv[1:])
+
+
+@pytest.mark.parametrize("nnew", [[2, 1, 1], [5, 40, 1]])
+def test_attn_of_a_part_of_a_batch(fnlib, nnew):
+    """The same for the attention: rows before cu[0] are no request's, nothing of them is written and nothing is wrong."""
+    _say("kv4 part", nnew)
+    c = Batch([20, 70, 33], nnew, nq=8, nkv=1, seed=38, pad=2)
+    og, cache = _run(fnlib, c, 2)
+    n, end = nnew[0], int(c.cu[-1])
+    before = c.cache
+    c.B, c.past, c.nnew, c.cu, c.full = 2, c.past[1:].copy(), c.nnew[1:].copy(), c.cu[1:].copy(), c.full[1:].copy()
+    c.seq = np.maximum(c.seq - 1, -1)
+    fnlib.dev_status()
+    part, pcache = _run(fnlib, c, 2)
+    assert fnlib.dev_status() == 0
+    assert (part[:n] == 7.5).all() and (part[end:] == 7.5).all()
+    ref = before.copy()
+    want = serve.attn_kv4(c.past, c.cu - n, c.full, c.slot[n:], c.qg[n:], c.k[n:], c.v[n:], c.wq, c.wk, ref)
+    assert np.array_equal(pcache, ref)
+    assert oracle.relerr(part[n:end], want) <= TOL
