@@ -4,6 +4,8 @@ a larger one, and what the status word says."""
 import numpy as np
 import pytest
 
+import fn
+import hiprt
 import oracle
 from oracle import serve
 from test_gpu_gdn_chunk import Block
@@ -187,3 +189,56 @@ def test_attn_of_a_part_of_a_batch(fnlib, nnew):
     want = serve.attn_kv4(c.past, c.cu - n, c.full, c.slot[n:], c.qg[n:], c.k[n:], c.v[n:], c.wq, c.wk, ref)
     assert np.array_equal(pcache, ref)
     assert oracle.relerr(part[n:end], want) <= TOL
+
+
+# what is wrong with a plan, and the bits that say so
+WRONG = {"nothing": 0, "pages": fn.STATUS_PAGE, "table": fn.STATUS_POS, "past": fn.STATUS_POS, "rows": fn.STATUS_ROWS,
+         "count": fn.STATUS_ROWS, "pages and table": fn.STATUS_PAGE | fn.STATUS_POS, "lost page": fn.STATUS_PAGE}
+
+
+# one workgroup for all tokens (up to 4096), many, and a second launch for the tokens (the count that is left in the place
+# that is read); requests whose past stays in the LDS (up to 5000) or not
+@pytest.mark.parametrize("wrong", list(WRONG))
+@pytest.mark.parametrize("B,T,in_place", [(9, 600, False), (9, 600, True), (9, 4500, False), (9, 4500, True), (5001, 5200, False)])
+def test_plan_says_what_is_wrong(fnlib, wrong, B, T, in_place):
+    """Exactly the bits of what is wrong, in every way that a plan is launched, and the tables of the plain form beside."""
+    _say("plan wrong", wrong, B, T, in_place)
+    r = np.random.default_rng(B + T)
+    past = r.integers(0, 200, B).astype(np.int32)
+    nnew = np.bincount(r.integers(0, B, T - 3), minlength=B).astype(np.int32)
+    past[2], nnew[2] = 100, 60
+    rows = T = int(nnew.sum()) + 3
+    want = (past + nnew + 63) // 64
+    have = (past + 63) // 64
+    mb = int(want.max())
+    if "table" in wrong:
+        mb -= 1
+    if wrong == "past":
+        past[2] = -4
+    if wrong == "count":
+        nnew[2] = -1
+    if wrong == "rows":
+        T = rows - 4
+    need = int((np.minimum(want, mb) - np.minimum(have, mb)).clip(0).sum())
+    npages = int(have.sum()) + need
+    order = r.permutation(npages).astype(np.int32)
+    have = np.minimum(have, mb)
+    table = np.full((B, mb), -1, np.int32)
+    table[np.arange(mb)[None] < have[:, None]] = order[:have.sum()]
+    free = np.full(npages, -1, np.int32)
+    free[:need] = order[have.sum():have.sum() + need]
+    top = need - (2 if "pages" in wrong else 0)
+    if wrong == "lost page":
+        table[2, 1] = -1      # its past ends in this block, and new tokens go on in it
+    z = lambda *n: np.zeros(n, np.int32) - 9  # noqa: E731
+    d = {k: hiprt.Buf.like(a) for k, a in dict(past=past, nnew=nnew, free=free, top=np.array([top], np.int32), left=z(1), table=table,
+                                               cu=z(B + 1), slot=z(T), seq=z(T)).items()}
+    left = d["top"] if in_place else d["left"]
+    fnlib.dev_status()
+    fnlib.page_plan_dev(B, T, mb, npages, d["past"].ptr, d["nnew"].ptr, d["free"].ptr, d["top"].ptr, left.ptr, d["table"].ptr,
+                        d["cu"].ptr, d["slot"].ptr, d["seq"].ptr)
+    hiprt.sync()
+    assert fnlib.dev_status() == WRONG[wrong]
+    ref = serve.plan(past, nnew, T, mb, free, top, table)
+    for got, x in zip((left, d["table"], d["cu"], d["slot"], d["seq"]), ref):
+        assert np.array_equal(got.download().reshape(np.shape(x)), x)
