@@ -912,7 +912,8 @@ int gdn_chunk_launch(const GdnChunk &p, hipStream_t st) {
     auto *scan = nc == 1 ? k_chunk_scan<1> : k_chunk_scan<2>;
     const size_t norm = ((size_t) p.T * p.nvh + 7) / 8;                                   // blocks of k_chunk_finish
     const size_t ring = p.B * ((((size_t) 2 * p.nkh + p.nvh) * D + 255) / 256);
-    if (norm + ring > 0x7fffffffu) FN_FAIL("gdn_chunk: too many rows");
+    // a launch has below 2^32 threads, 256 a workgroup
+    if (items > 0xffffffu || (block && norm + ring > 0xffffffu)) FN_FAIL("gdn_chunk: too many rows");
     if (block) {
         hipLaunchKernelGGL(k_chunk_intra<true>, gi, dim3(256), 0, st, a);
         hipLaunchKernelGGL(scan, gs, dim3(576), 0, st, a);

@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(128) k_kv4_unpack(const Kv4Rows p) {
 int check(const Kv4Rows &p) {
     if (p.n < 1 || p.nkv < 1) FN_FAIL("kv4: n and nkv must be >= 1");
     if (p.nkv > 65535) FN_FAIL("kv4: nkv must be <= 65535");
+    if (p.n > (1 << 25) - 1) FN_FAIL("kv4: n must be <= 33554431 (a launch has below 2^32 threads)");
     if (p.hd != HD) FN_FAIL("kv4: only head_dim 256 is built");
     if (p.npages < 1 || p.npages > INT_MAX / PG) FN_FAIL("kv4: npages must be in 1..33554431 (slots are 32-bit)");
     if (!p.slot || !p.k || !p.v || !p.cache) FN_FAIL("kv4: null pointer");

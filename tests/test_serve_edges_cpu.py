@@ -40,3 +40,19 @@ def test_performance_cases_call_what_there_is():
         inspect.signature(getattr(fn.FN, node.func.attr)).bind(None, *[0] * _places(node), **{k.arg: 0 for k in node.keywords})
         seen.add(node.func.attr)
     assert {"page_plan_dev", "attn_kv4_dev", "gdn_chunk_work_bytes", "gdn_core_chunk_dev", "gdn_block_chunk_dev"} <= seen
+
+
+@pytest.mark.parametrize("call", ["kv4_pack_dev", "kv4_unpack_dev"])
+def test_more_rows_than_a_launch_has_are_refused(fnlib, call):
+    with pytest.raises(RuntimeError, match="n must be <= 33554431"):
+        getattr(fnlib, call)(1 << 25, 1, 4, 4096, *[4096] * 3)
+
+
+def test_more_chunks_than_a_launch_has_are_refused(fnlib):
+    """Before any work is launched: workgroups of the preparation, and of the block's gated norm."""
+    T, p = 1 << 30, 4096
+    with pytest.raises(RuntimeError, match="too many rows"):
+        fnlib.gdn_core_chunk_dev(1, T, 1, 1, *[p] * 9, 1 << 60)
+    T = 1 << 23
+    with pytest.raises(RuntimeError, match="too many rows"):
+        fnlib.gdn_block_chunk_dev(1, T, 1, 16, 4, *[p] * 13, 1 << 60)
