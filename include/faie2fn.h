@@ -342,8 +342,10 @@ int fn_attn_kv4_nsplit(int B, int T, int nq, int nkv, int ctx);
 /* The DeltaNet core of fn_gdn_core_dev over a packed batch of prompts, 64 tokens at a time: q, k [T][nkh][dk],
  * v [T][nvh][dv], beta, g [T][nvh], cu [B + 1], S [B][nvh][dk][dv] in/out, o [T][nvh][dv].  The state of a request without
  * new tokens is left as it was.  An infinity or NaN in a request's inputs may reach all outputs of its value head from
- * the start of the 64 tokens that hold it.  q, k, o and work 16-byte aligned; work: fn_gdn_chunk_work_bytes(B, T, nkh, nvh)
- * bytes.  nvh up to 32768.  For one or a few tokens a request fn_gdn_core_dev and fn_gdn_block_dev are the faster calls. */
+ * the start of the 64 tokens that hold it.  A column (of v, of the state) keeps 2^-39 of its largest value or update in 64
+ * tokens: 24 bits of what is up to 2^15 below that, and fewer of what is less (values that differ by 10^6 among neighbours:
+ * take fn_gdn_core_dev, which rounds each token by itself).  q, k, o and work 16-byte aligned; work:
+ * fn_gdn_chunk_work_bytes(B, T, nkh, nvh) bytes.  nvh up to 32768.  For one or a few tokens a request fn_gdn_core_dev and fn_gdn_block_dev are the faster calls. */
 int fn_gdn_core_chunk_dev(int B, int T, int nkh, int nvh, int dk, int dv, int head_map, const int32_t *cu, const float *q,
                           const float *k, const float *v, const float *beta, const float *g, float *S, float *o,
                           void *work, size_t work_bytes, void *stream);

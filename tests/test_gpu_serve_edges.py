@@ -8,7 +8,7 @@ import fn
 import hiprt
 import oracle
 from oracle import serve
-from test_gpu_gdn_chunk import Block
+from test_gpu_gdn_chunk import Block, Core
 from test_gpu_serve import TOL, Batch, _run, _say
 
 pytestmark = pytest.mark.gpu
@@ -242,3 +242,28 @@ def test_plan_says_what_is_wrong(fnlib, wrong, B, T, in_place):
     ref = serve.plan(past, nnew, T, mb, free, top, table)
     for got, x in zip((left, d["table"], d["cu"], d["slot"], d["seq"]), ref):
         assert np.array_equal(got.download().reshape(np.shape(x)), x)
+
+
+@pytest.mark.parametrize("forget", [False, True])
+@pytest.mark.parametrize("jump", [1e4, 1e6, 1e8, 1e12])
+def test_core_values_that_fall(fnlib, jump, forget):
+    """Values that fall within a chunk, with the ordinary decays and with one of 0 at the fall.  A column's operands are
+    rounded at 2^-39 of its largest value or update; a row of M and of P sums 64 such with factors of 1 at most and 2^2.5
+    in all for keys of random directions, one after the other: 2^-34 of the largest value.  What comes before the fall is at
+    the bar."""
+    _say("core fall", jump, forget)
+    c = Core([64, 100], seed=40)
+    fall = [32, 64 + 40]
+    for a, b in ((0, fall[0]), (64, fall[1])):
+        c.v[a:b] *= np.float32(jump)
+    if forget:
+        c.g[fall] = -np.inf
+    o, S = c.run(fnlib)
+    ro, rS = c.reference()
+    top = np.abs(c.v).max()
+    assert np.abs(o - ro).max() <= max(2.0 ** -34 * top, TOL * np.abs(ro).max())
+    for a, b in ((0, fall[0]), (64, fall[1])):
+        assert oracle.relerr(o[a:b], ro[a:b]) <= TOL
+    for a, b in ((fall[0], 64), (fall[1], 128)):
+        assert np.abs(o[a:b] - ro[a:b]).max() <= 2.0 ** -34 * top + TOL * np.abs(ro[a:b]).max()
+    assert np.abs(S[0] - rS[0]).max() <= 2.0 ** -34 * top + TOL * np.abs(rS[0]).max()
