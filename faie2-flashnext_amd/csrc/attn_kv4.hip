@@ -941,7 +941,9 @@ size_t kv4_work_bytes(int B, int T, int nq, int nkv, int hd, int nsplit) {
 
 int kv4_pick_nsplit(int B, int T, int nq, int nkv, int ctx) {
     const int grp = nq / nkv, rt = item_rows(B, T, grp);
-    // one round of workgroups, two a CU: items of an average request times requests
+    // One round of workgroups, two a CU (k_attn_kv4 has room for three; what that gives was measured for one request only,
+    // below): items of an average request times requests.  All requests of a call get as many splits, so a long one among
+    // short ones or beside prompts is the call's time.
     const long long avg = ((long long) T * grp + B - 1) / B, groups = std::max(1ll, (avg + rt - 1) / rt) * B * nkv;
     const long long want = std::max(1ll, 2ll * device_cus() / groups);
     // A split costs a row of sums that is written and read again, so the time is about u keys / nsplit + w nsplit, least at

@@ -281,7 +281,8 @@ int fn_test_attn_qsa(int B, int nq, int nkv, int hd, int nrot, float theta, floa
  * 3c. Serving a packed batch (new; no counterpart in the reference, which decodes one sequence): requests of different
  *     lengths in one call.  Request b's new tokens are rows cu[b] .. cu[b + 1] - 1 of every per-token array of T rows; rows
  *     before cu[0] and from cu[B] on are left as they were (a call may take a run of a batch's requests: cu + i, and the
- *     arrays of B entries from i on, seq counted from i).  past [B] are the tokens that each request already has (0 for a new one).
+ *     arrays of B entries from i on, seq counted from i).  past [B] are the tokens that each request already has (0 for a
+ *     new one).
  *     Nothing is allocated and no memset is recorded; a call can be captured into a graph and replayed with new
  *     contents of its buffers.  A workspace holds nothing between calls; calls that may run at the same time (two streams,
  *     two graphs) need one each.  All buffers are on the device that is current at the call.  cu does not decrease.  What
@@ -313,8 +314,8 @@ int fn_page_release_dev(int B, int max_blocks, int npages, const int32_t *done, 
 size_t fn_kv4_page_bytes(int nkv, int hd);
 
 /* Rows k, v [n][nkv][hd] (keys already normalised and rotated) into slots slot [n], and back as the values that they stand
- * for; n below 2^25.  A slot of -1 is passed over (unpack leaves its row as it was).  k, v and cache 16-byte aligned; the slots of one
- * pack are different. */
+ * for; n below 2^25.  A slot of -1 is passed over (unpack leaves its row as it was).  k, v and cache 16-byte aligned; the
+ * slots of one pack are different. */
 int fn_kv4_pack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, const float *k, const float *v,
                     uint8_t *cache, void *stream);
 int fn_kv4_unpack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, const uint8_t *cache, float *k, float *v,
@@ -325,13 +326,15 @@ int fn_kv4_unpack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, c
  * past[b] + t - cu[b]: its normalised, rotated key and its value are written to slot[t] in 4 bits; its queries attend
  * the request's keys up to its own position as the cache holds them (a block whose table entry is outside the cache is
  * passed over; a query that finds no key gets zeros).  The rotation's angle is taken in 64 bits.  nq / nkv any whole number.
- * Sums are in fp32: of any values of the cache over up to 2^19 keys of a query, of values below 2^117 over any number.  A score
- * q.k that fp32 does not hold (packed keys near its end) may make the output NaN.
- * nsplit: key splits of a row (fn_attn_kv4_nsplit: the choice for contexts of up to ctx keys).  All arrays but the
+ * Sums are in fp32: of any values of the cache over up to 2^19 keys of a query, of values below 2^117 over any number.  A
+ * score q.k that fp32 does not hold (packed keys near its end) may make the output NaN.
+ * nsplit: key splits of a row, of every request (fn_attn_kv4_nsplit: the choice for contexts of up to ctx keys and
+ * requests alike; decode steps over long contexts are best not in one call with prompts).  All arrays but the
  * int32 ones 16-byte aligned; work: fn_attn_kv4_work_bytes() bytes.  The slots of one call (other than -1) are different.
  * T nq / nkv / 32 + B (in batches of up to 24 nkv / nq rows a request: / 8) is at most 65535.
  * Requests may name the same pages in their tables.  A row whose seq is not the request whose rows it lies in is not
- * cached, its output is undefined, and the status word says so. */
+ * cached, and the status word says so; its request's outputs are then undefined, as they are where a row has slot -1 and
+ * the table a page for it: such a key is whatever the page holds there. */
 int fn_attn_kv4_dev(int B, int T, int nq, int nkv, int hd, int nrot, float theta, float eps, int max_blocks, int npages,
                     const int32_t *past, const int32_t *cu, const int32_t *table, const int32_t *slot,
                     const int32_t *seq, const float *qg, const float *k, const float *v, const float *wq,
@@ -345,7 +348,8 @@ int fn_attn_kv4_nsplit(int B, int T, int nq, int nkv, int ctx);
  * the start of the 64 tokens that hold it.  A column (of v, of the state) keeps 2^-39 of its largest value or update in 64
  * tokens: 24 bits of what is up to 2^15 below that, and fewer of what is less (values that differ by 10^6 among neighbours:
  * take fn_gdn_core_dev, which rounds each token by itself).  q, k, o and work 16-byte aligned; work:
- * fn_gdn_chunk_work_bytes(B, T, nkh, nvh) bytes.  nvh up to 32768.  For one or a few tokens a request fn_gdn_core_dev and fn_gdn_block_dev are the faster calls. */
+ * fn_gdn_chunk_work_bytes(B, T, nkh, nvh) bytes.  nvh up to 32768.  For one or a few tokens a request fn_gdn_core_dev and
+ * fn_gdn_block_dev are the faster calls. */
 int fn_gdn_core_chunk_dev(int B, int T, int nkh, int nvh, int dk, int dv, int head_map, const int32_t *cu, const float *q,
                           const float *k, const float *v, const float *beta, const float *g, float *S, float *o,
                           void *work, size_t work_bytes, void *stream);
