@@ -24,11 +24,14 @@ __global__ void __launch_bounds__(128) k_kv4_pack(const Kv4Rows p, unsigned *sta
     else store_row<true>(page, slot % PG, y, lane, status);
 }
 
-__global__ void __launch_bounds__(128) k_kv4_unpack(const Kv4Rows p) {
+__global__ void __launch_bounds__(128) k_kv4_unpack(const Kv4Rows p, unsigned *status) {
     const int i = blockIdx.x, g = blockIdx.y, lane = threadIdx.x & 63, grp = lane >> 3, sub = lane & 7;
     const bool is_v = threadIdx.x >= 64;
     const int slot = p.slot[i];
-    if (slot < 0 || slot / PG >= p.npages) return;
+    if (slot < 0 || slot / PG >= p.npages) {
+        if (slot >= 0 && threadIdx.x == 0) atomicOr(status, FN_STATUS_PAGE);
+        return;
+    }
     const uint8_t *page = p.cache + ((size_t) (slot / PG) * p.nkv + g) * HEAD_BYTES;
     const int r = slot % PG;
     uint32_t c;
@@ -70,7 +73,9 @@ int kv4_pack_launch(const Kv4Rows &p, hipStream_t st) {
 
 int kv4_unpack_launch(const Kv4Rows &p, hipStream_t st) {
     if (check(p)) return -1;
-    hipLaunchKernelGGL(k_kv4_unpack, dim3(p.n, p.nkv), dim3(128), 0, st, p);
+    unsigned *status;
+    if (status_word(&status)) return -1;
+    hipLaunchKernelGGL(k_kv4_unpack, dim3(p.n, p.nkv), dim3(128), 0, st, p, status);
     FN_CK(hipGetLastError());
     return 0;
 }

@@ -314,8 +314,8 @@ int fn_page_release_dev(int B, int max_blocks, int npages, const int32_t *done, 
 size_t fn_kv4_page_bytes(int nkv, int hd);
 
 /* Rows k, v [n][nkv][hd] (keys already normalised and rotated) into slots slot [n], and back as the values that they stand
- * for; n below 2^25.  A slot of -1 is passed over (unpack leaves its row as it was).  k, v and cache 16-byte aligned; the
- * slots of one pack are different. */
+ * for; n below 2^25.  A slot of -1 is passed over (unpack leaves its row as it was), one outside the cache too, and the
+ * status word says so.  k, v and cache 16-byte aligned; the slots of one pack are different. */
 int fn_kv4_pack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, const float *k, const float *v,
                     uint8_t *cache, void *stream);
 int fn_kv4_unpack_dev(int n, int nkv, int hd, int npages, const int32_t *slot, const uint8_t *cache, float *k, float *v,

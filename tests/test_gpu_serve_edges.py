@@ -267,3 +267,21 @@ def test_core_values_that_fall(fnlib, jump, forget):
     for a, b in ((fall[0], 64), (fall[1], 128)):
         assert np.abs(o[a:b] - ro[a:b]).max() <= 2.0 ** -34 * top + TOL * np.abs(ro[a:b]).max()
     assert np.abs(S[0] - rS[0]).max() <= 2.0 ** -34 * top + TOL * np.abs(rS[0]).max()
+
+
+def test_unpack_says_that_a_slot_is_outside(fnlib):
+    """As packing does; a slot of -1 is no mistake.  Either way the row is left as it was."""
+    _say("unpack outside")
+    npages, n = 2, 4
+    slot = np.array([5, -1, 127, -1], np.int32)
+    cache = hiprt.Buf.like(np.full((npages, 1, serve.HEAD_BYTES), 127, np.uint8))
+    k, v = (hiprt.Buf.like(np.full((n, 1, 256), 9.0, np.float32)) for _ in range(2))
+    fnlib.dev_status()
+    for bad, bits in ((-1, 0), (npages * 64, fn.STATUS_PAGE), (2 ** 31 - 1, fn.STATUS_PAGE)):
+        slot[3] = bad
+        d = hiprt.Buf.like(slot)
+        fnlib.kv4_unpack_dev(n, 1, npages, d.ptr, cache.ptr, k.ptr, v.ptr)
+        hiprt.sync()
+        assert fnlib.dev_status() == bits, bad
+        for x in (k.download(), v.download()):
+            assert (x[[1, 3]] == 9.0).all() and (np.abs(x[[0, 2]]) == 6.0).all()    # (codes 7 and 15, scale 1)
